@@ -32,7 +32,9 @@ ARCH = "gfx950"
 HIP_SOURCES = ["attn_fwd_mfma16.hip", "attn_fwd_pipe16_f16.hip", "attn_fwd_pipe16_f16ps.hip",
                "attn_fwd_pipe16_bf16.hip", "attn_fwd_plan16.hip", "attn_fwd_pipe16w.hip", "attn_fwd_pipe16wm.hip", "attn_fwd_pipe16b.hip",
                "attn_fwd_mask_bits.hip", "attn_fwd_short16.hip", "attn_fwd_mfma32.hip",
-               "attn_fwd_decode16.hip", "attn_bwd16.hip", "attn_bwd32.hip", "attn_abi.cpp"]
+               "attn_fwd_decode16.hip", "attn_bwd16.hip", "attn_bwd32.hip", "attn_abi.cpp",
+               "paged_append.hip", "paged_attn.hip", "paged_select.hip", "paged_abi.cpp"]
+NATIVE_SOURCES = ["main.cpp", "paged_binding.cpp"]
 HIP_FLAGS = [
     f"--offload-arch={ARCH}", "-O3", "-std=c++17", "-fPIC", "-Wall",
     "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops",
@@ -51,7 +53,11 @@ FILE_FLAGS_DROP = {"attn_fwd_pipe16_f16.hip": {"-mno-amdgpu-ieee", "-fno-honor-n
                    "attn_fwd_pipe16_bf16.hip": {"-mno-amdgpu-ieee", "-fno-honor-nans"},
                    "attn_fwd_pipe16w.hip": {"-mno-amdgpu-ieee", "-fno-honor-nans"},
                    "attn_fwd_pipe16wm.hip": {"-mno-amdgpu-ieee", "-fno-honor-nans"},
-                   "attn_fwd_pipe16b.hip": {"-mno-amdgpu-ieee", "-fno-honor-nans"}}
+                   "attn_fwd_pipe16b.hip": {"-mno-amdgpu-ieee", "-fno-honor-nans"},
+                   # the paged kernels' bounds, orders and error rows rely on NaN
+                   "paged_append.hip": {"-mno-amdgpu-ieee", "-fno-honor-nans"},
+                   "paged_attn.hip": {"-mno-amdgpu-ieee", "-fno-honor-nans"},
+                   "paged_select.hip": {"-mno-amdgpu-ieee", "-fno-honor-nans"}}
 
 LIB_NAME = "libcmpext3_attn.so"
 
@@ -101,7 +107,7 @@ def build_native(verbose: bool) -> str:
     tmp = out + ".tmp"
     abi = int(torch._C._GLIBCXX_USE_CXX11_ABI)
     cxx = os.environ.get("CXX", shutil.which("g++") or "g++")
-    cmd = [cxx, "-O2", "-std=c++17", "-fPIC", "-shared", os.path.join(CSRC, "main.cpp"), "-o", tmp,
+    cmd = [cxx, "-O2", "-std=c++17", "-fPIC", "-shared", *(os.path.join(CSRC, f) for f in NATIVE_SOURCES), "-o", tmp,
            *[f"-I{p}" for p in cpp_extension.include_paths()], f"-I{py_inc}", f"-I{ROCM}/include",
            f"-I{INCLUDE}",
            "-D__HIP_PLATFORM_AMD__=1", "-DUSE_ROCM=1", "-DTORCH_EXTENSION_NAME=_native",

@@ -62,7 +62,8 @@ ops = _C
 from . import autoselect  # noqa: E402
 
 __all__ = ["enable", "disable", "is_enabled", "autoselect_report", "ops", "autoselect",
-           "attention", "enable_backward", "backward_enabled"]
+           "attention", "enable_backward", "backward_enabled",
+           "paged_append", "paged_attention", "paged_select"]
 
 _SUPPORTED_DTYPES = (torch.float16, torch.float32, torch.bfloat16)
 _ORIGINALS: dict[tuple[Any, str], Callable] = {}
@@ -181,6 +182,55 @@ def attention(query: torch.Tensor, key: torch.Tensor, value: torch.Tensor,
     torch's enable_gqa meaning; attn_mask as in SDPA, bool or additive, no
     gradient taken for it).  Raises RuntimeError for anything else."""
     return _Attention.apply(query, key, value, scale, causal, attn_mask)
+
+
+def paged_append(key: torch.Tensor, value: torch.Tensor, key_pages: torch.Tensor,
+                 value_pages: torch.Tensor, page_table: torch.Tensor, seq_lens: torch.Tensor, *,
+                 query: torch.Tensor | None = None, cos: torch.Tensor | None = None,
+                 sin: torch.Tensor | None = None, positions: torch.Tensor | None = None,
+                 new_lens: torch.Tensor | None = None, interleaved: bool = False,
+                 key_bounds: torch.Tensor | None = None) -> torch.Tensor | None:
+    """Store new tokens' key and value [B, Hkv, S, D] in a paged cache, in place,
+    and return their queries rotated (None without `query`).
+
+    key_pages, value_pages  [pages, Hkv, page_size, D], any strides in whole 16-byte chunks
+    page_table   int32 [B, pages of a sequence]; token j is in page page_table[b, j // page_size]
+    seq_lens     int32 [B], the tokens of each sequence, the new ones among them; 0: no sequence here
+    new_lens     int32 [B]: column i < new_lens[b] holds token seq_lens[b] - new_lens[b] + i, later
+                 columns are padding; by default every column is new (the first seq_lens[b], if fewer)
+    cos, sin     fp32 [rows, R / 2]: keys and queries [B, H, S, D] are rotated in their first R dims by
+                 row positions[b, i] (int32 [B, S]; the token's place in its sequence by default), as
+                 pairs (d, d + R/2), or (2d, 2d + 1) when `interleaved`
+    key_bounds   [pages, Hkv, 2, D]: every channel's lowest and highest key of a page, kept up to date
+                 for paged_select
+
+    Padding columns of the result are zero.  A token without a valid page or rotation row is not
+    stored and its query row is NaN.  No gradient: calls under live autograd raise RuntimeError, as
+    does anything the kernels cannot take."""
+    return _C.paged_append(key, value, key_pages, value_pages, page_table, seq_lens, query, cos, sin,
+                           positions, new_lens, interleaved, key_bounds)
+
+
+def paged_attention(query: torch.Tensor, key_pages: torch.Tensor, value_pages: torch.Tensor,
+                    page_table: torch.Tensor, seq_lens: torch.Tensor, scale: float | None = None, *,
+                    new_lens: torch.Tensor | None = None,
+                    selected: torch.Tensor | None = None) -> torch.Tensor:
+    """softmax(scale * Q K^T) V of new tokens' queries [B, H, S, D] (S <= 16) over a paged cache, which
+    holds them already (paged_append; same page_table, seq_lens and new_lens).  A token sees its own
+    key and those before it; K/V may hold fewer heads than Q.  With `selected` (int32 [B, Hkv, n],
+    columns of page_table, negative entries left out) each K/V head attends to those pages only.
+    Padding columns and places without a sequence give zeros; a page number outside the pool, or a
+    sequence longer than its table row, gives NaN rows.  No gradient."""
+    return _C.paged_attention(query, key_pages, value_pages, page_table, seq_lens, scale, new_lens, selected)
+
+
+def paged_select(query: torch.Tensor, key_bounds: torch.Tensor, page_table: torch.Tensor,
+                 seq_lens: torch.Tensor, page_size: int, n_selected: int) -> torch.Tensor:
+    """The pages each sequence's new token (query [B, H, 1, D]) should attend to: int32 [B, Hkv,
+    n_selected], ascending, -1 behind the last.  The page of the newest token is among them; the
+    others are those whose key_bounds allow the largest sum of q k over the head group's queries
+    (64-bit scores; the lower page of equals)."""
+    return _C.paged_select(query, key_bounds, page_table, seq_lens, page_size, n_selected)
 
 
 def _training_applies(query, key, value, attn_mask, dropout_p, enable_gqa) -> bool:

@@ -13,13 +13,15 @@ from typing import Optional
 
 LIB_PATH = os.path.join(os.path.dirname(os.path.abspath(__file__)), "libcmpext3_attn.so")
 
-# Every function include/cmpext3_attn.h declares.
+# Every function include/cmpext3_attn.h and include/cmpext3_paged.h declare.
 SYMBOLS = ("cmpext3_attn_fwd", "cmpext3_attn_fwd_gqa", "cmpext3_attn_fwd_masked",
            "cmpext3_attn_fwd_ws", "cmpext3_attn_fwd_workspace_size", "cmpext3_attn_fwd_plan",
            "cmpext3_attn_fwd_mask_workspace_size",
            "cmpext3_attn_fwd_noalloc", "cmpext3_attn_fwd_lse", "cmpext3_attn_bwd",
            "cmpext3_attn_bwd_ws", "cmpext3_attn_bwd_workspace_size",
-           "cmpext3_attn_strerror", "cmpext3_attn_abi_version", "cmpext3_attn_describe")
+           "cmpext3_attn_strerror", "cmpext3_attn_abi_version", "cmpext3_attn_describe",
+           "cmpext3_paged_append", "cmpext3_paged_attn", "cmpext3_paged_attn_workspace_size",
+           "cmpext3_paged_select", "cmpext3_paged_select_workspace_size")
 
 DTYPE_F16, DTYPE_BF16, DTYPE_F32, DTYPE_BOOL = 0, 1, 2, 3
 WORKSPACE_COUNTER_BYTES = 65536                     # CMPEXT3_WORKSPACE_COUNTER_BYTES
@@ -74,6 +76,19 @@ def lib() -> ctypes.CDLL:
         L.cmpext3_attn_bwd_ws.restype = ci
         L.cmpext3_attn_bwd_workspace_size.argtypes = [ci] * 9
         L.cmpext3_attn_bwd_workspace_size.restype = sz
+        i64 = ctypes.c_int64
+        L.cmpext3_paged_append.argtypes = ([vp] * 7 + [ci] * 8 + [i64p] * 7 + [vp, ci, i64] + [vp] * 5
+                                           + [ci, ci, i64, ci, vp])
+        L.cmpext3_paged_append.restype = ci
+        L.cmpext3_paged_attn.argtypes = ([vp] * 4 + [ci] * 8 + [i64p] * 4 + [vp, ci, i64] + [vp] * 3
+                                         + [ci, ctypes.c_float, vp, sz, vp])
+        L.cmpext3_paged_attn.restype = ci
+        L.cmpext3_paged_attn_workspace_size.argtypes = [ci] * 9
+        L.cmpext3_paged_attn_workspace_size.restype = sz
+        L.cmpext3_paged_select.argtypes = ([vp] * 3 + [ci] * 7 + [i64p] * 2 + [vp, ci, i64, vp, ci, vp, sz, vp])
+        L.cmpext3_paged_select.restype = ci
+        L.cmpext3_paged_select_workspace_size.argtypes = [ci] * 3
+        L.cmpext3_paged_select_workspace_size.restype = sz
         L.cmpext3_attn_strerror.argtypes = [ci]
         L.cmpext3_attn_strerror.restype = ctypes.c_char_p
         L.cmpext3_attn_abi_version.argtypes = []

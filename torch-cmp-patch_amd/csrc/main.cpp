@@ -35,13 +35,11 @@
 #include <utility>
 #include <vector>
 
-#include <torch/extension.h>
-#include <ATen/hip/impl/HIPGuardImplMasqueradingAsCUDA.h>
-#include <ATen/hip/impl/HIPStreamMasqueradingAsCUDA.h>
+#include "binding.h"
 
 #include "../../include/cmpext3_attn.h"
 
-namespace {
+namespace cmpext3_binding {
 
 int dtype_code(at::ScalarType t) {
   switch (t) {
@@ -52,24 +50,17 @@ int dtype_code(at::ScalarType t) {
   }
 }
 
+}  // namespace cmpext3_binding
+
+using namespace cmpext3_binding;
+
+namespace {
+
 // attention mask in the form the C ABI takes: [B,H,Sq,Sk] view, unit key
 // stride, other strides multiples of 4 elements (0 = broadcast)
 struct Mask {
   torch::Tensor t;
   int dtype = -1;
-};
-
-// Key-split workspace of one (device, stream): a byte tensor from torch's
-// caching allocator (so torch.cuda.memory_allocated counts it), zero-filled
-// when made -- its first 64 KiB are the counters every launch leaves at zero
-// -- and kept for later calls on the stream, replaced by a larger one when a
-// bigger plan arrives.  Calls on one stream run in order, so they can share
-// it.  A stream under graph capture gets none and its launch runs unsplit: a
-// captured launch would carry the buffer into replays that can run beside
-// eager calls on the stream.
-struct Workspace {
-  void* ptr = nullptr;
-  size_t bytes = 0;
 };
 
 std::mutex ws_mu;
@@ -82,6 +73,10 @@ std::map<std::pair<int, hipStream_t>, torch::Tensor> ws_cache;  // guarded by ws
 // over 100 MB of mask).
 constexpr size_t kKeptMaskBits = size_t(16) << 20;
 constexpr size_t kWorkspaceStep = size_t(4) << 20;
+
+}  // namespace
+
+namespace cmpext3_binding {
 
 bool capturing(hipStream_t stream) {
   hipStreamCaptureStatus cap = hipStreamCaptureStatusNone;
@@ -103,6 +98,10 @@ Workspace workspace_for(const torch::Tensor& like, hipStream_t stream, size_t ne
   w.bytes = (size_t)t.numel();
   return w;
 }
+
+}  // namespace cmpext3_binding
+
+namespace {
 
 size_t workspace_size_of(int device, hipStream_t stream) {
   std::lock_guard<std::mutex> lock(ws_mu);
@@ -471,4 +470,5 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("workspace_bytes", &workspace_bytes,
         "Bytes of key-split workspace the binding keeps for the current stream of `device` (0: none yet)",
         py::arg("device") = 0);
+  register_paged(m);
 }
