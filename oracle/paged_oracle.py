@@ -81,7 +81,7 @@ def attention(query, key_pages, value_pages, table, lens, scale, new_lens=None, 
     for b in range(B):
         n, length = new_count(b, S, lens, new_lens), max(int(lens[b]), 0)
         pages = -(-length // page_size)
-        for hk in range(Hkv):
+        for hk in range(Hkv if n else 0):  # only padding: zeros
             cols = range(pages) if selected is None else [int(x) for x in selected[b, hk] if int(x) >= 0]
             at = [page_of(table, b, c, P) if c < pages else None for c in cols]
             heads = slice(hk * H // Hkv, (hk + 1) * H // Hkv)
