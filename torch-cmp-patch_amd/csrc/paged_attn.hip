@@ -21,9 +21,9 @@
 //    load of the table per 64 tiles, checked there), read back by v_readlane.
 //  * Scores S^T = K Q^T and O^T = V^T P^T on 16x16 MFMAs (16x16x32 and 16x16x16
 //    for fp16 and bf16, 16x16x4 for fp32), exact online softmax in the exp2
-//    domain with fp32 state.  For fp16 and bf16 the weights are rounded to the
-//    tensors' type for the second product; their sum takes the rounded values,
-//    so the weights still add up to 1.
+//    domain with fp32 state.  For fp16 and bf16 a weight enters the second
+//    product in two parts, its value rounded to the tensors' type and the
+//    rounded rest (the matrix units are idle for most of the time anyway).
 //  * End of a segment: the waves' (O, m, l) meet in LDS.  A unit that is one
 //    segment is written out; otherwise each of its workgroups leaves its part
 //    in the workspace and counts itself in, and the last one joins the parts in
@@ -52,8 +52,10 @@ template <> struct Mma<_Float16> {
   static __device__ __forceinline__ uint32_t pack(float a, float b) {
     return __builtin_bit_cast(uint32_t, __builtin_convertvector((f32x2p){a, b}, f16x2p));
   }
-  static __device__ __forceinline__ float sum2(uint32_t w, float acc) {
-    return __builtin_amdgcn_fdot2(__builtin_bit_cast(f16x2p, w), (f16x2p){1.0f16, 1.0f16}, acc, false);
+  // what rounding a and b to w left, rounded
+  static __device__ __forceinline__ uint32_t rest(uint32_t w, float a, float b) {
+    const f16x2p h = __builtin_bit_cast(f16x2p, w);
+    return pack(a - (float)h[0], b - (float)h[1]);
   }
 };
 template <> struct Mma<__bf16> {
@@ -66,9 +68,8 @@ template <> struct Mma<__bf16> {
   static __device__ __forceinline__ uint32_t pack(float a, float b) {
     return __builtin_bit_cast(uint32_t, __builtin_convertvector((f32x2p){a, b}, bf16x2p));
   }
-  static __device__ __forceinline__ float sum2(uint32_t w, float acc) {
-    const bf16x2p one = {(__bf16)1.0f, (__bf16)1.0f};
-    return __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(bf16x2p, w), one, acc, false);
+  static __device__ __forceinline__ uint32_t rest(uint32_t w, float a, float b) {
+    return pack(a - __uint_as_float(w << 16), b - __uint_as_float(w & 0xffff0000u));
   }
 };
 
@@ -76,6 +77,7 @@ constexpr int kRows = 16;        // query rows of a unit at most
 constexpr int kTile = 16;        // slots of a tile
 constexpr int kMaxWgs = 1024;    // workgroups of a launch at most (counters: one each)
 constexpr int kMinTiles = 16;    // tiles of a workgroup's share at least
+constexpr int kWhole = 32;       // tiles of a unit that is never split
 constexpr int kMergeLoads = 8;   // loads of one merging thread in flight together
 
 // Waves per workgroup and stages per wave: as many stages as 128 KB of LDS
@@ -94,21 +96,40 @@ __device__ __forceinline__ int pg_swz(int r, int c, int nc) {
   return c < (nc & ~7) ? (c ^ f) : c;
 }
 
+// lds_dma16 of a buffer whose descriptor a v_readlane may just have written (the
+// tile's own, or one that the compiler brings back from a lane): a vector
+// instruction's SGPR is not there for a memory instruction before five wait
+// states have passed, and the compiler does not see into the assembly.
+__device__ __forceinline__ void lds_dma16_fresh(const u32x4& rs, uint32_t lds_byte, int voff) {
+  asm volatile("s_nop 4\n\tbuffer_load_dwordx4 %0, %1, 0 offen lds" ::"v"(voff), "s"(rs), "{m0}"(lds_byte) : "memory");
+}
+
 struct Plan {
   f32x4* ws;  // parts: [workgroup][first or last segment][row] (DK / 4 + 1) float4: O, then (m, l, 0, 0)
   int* cnt;   // a counter for the unit that a workgroup's last segment begins
   int split;  // 0: whole units, dealt out in turn
+  int group;  // query heads per K/V head
+  int blocks; // row blocks per (sequence, K/V head)
+  int units;  // of a sequence
+  int tpp;    // tiles per page
 };
 
-// Tiles of sequence b, 0 when nothing of it is read (no tokens, no new ones, or
-// longer than its table row).
+// A sequence as the launch sees it.
+struct Seq {
+  int len, fresh;  // tokens, new ones among the columns
+  int tiles;       // 0: nothing of it is read (no tokens, no new ones, or longer than its table row)
+};
 template <bool SEL>
-__device__ __forceinline__ int tiles_of(const PagedAttnParams& p, int b, int tpp) {
-  const int len = seq_len_held(p.map, b), ps = p.map.page_size;
-  if (len == 0 || seq_new(p.map, b, p.S, len) == 0 || len > p.map.width * ps) return 0;
-  if (SEL) return p.n_selected * tpp;
-  const int full = len / ps;
-  return full * tpp + (len - full * ps + kTile - 1) / kTile;
+__device__ __forceinline__ Seq seq_of(const PagedAttnParams& p, int b, int tpp) {
+  Seq s;
+  const int ps = p.map.page_size;
+  s.len = seq_len_held(p.map, b);
+  s.fresh = seq_new(p.map, b, p.S, s.len);
+  if (s.fresh == 0 || s.len > p.map.width * ps) s.tiles = 0;
+  else if (SEL) s.tiles = p.n_selected * tpp;
+  else if (tpp * kTile == ps) s.tiles = (s.len + kTile - 1) / kTile;
+  else s.tiles = s.len / ps * tpp + (s.len % ps + kTile - 1) / kTile;
+  return s;
 }
 
 __device__ __forceinline__ float xor_f(float x, int m) { return __shfl_xor(x, m); }
@@ -133,73 +154,95 @@ __global__ __launch_bounds__(pg_waves(DK * sizeof(T)) * 64, 1) void paged_attn(P
   static_assert(NS >= 1 && IPT * (NS - 1) <= 63, "vmcnt range");
   static_assert(NW * kRows * MOS * 4 + 2 * NW * kRows * 4 + 16 <= RING, "the waves' states fit the ring");
   __shared__ __attribute__((aligned(16))) unsigned char lds[RING];
-  __shared__ int64_t s_wsum[NW];
-  __shared__ int64_t s_at[2];
-  __shared__ int s_b, s_flag;
+  __shared__ int s_flag;
 
   const int tid = thread_x(), lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int wg = block_x(), nwg = (int)gridDim.x;
   const int c = lane & 15, g = lane >> 4;
-  const int G = p.H / p.Hkv, rows_all = G * p.S, RBLK = (rows_all + kRows - 1) / kRows;
-  const int U = p.Hkv * RBLK;           // units of a sequence
-  const int ps = p.map.page_size, tpp = (ps + kTile - 1) / kTile;
+  const int G = a.group, rows_all = G * p.S, U = a.units;
+  const int ps = p.map.page_size, tpp = a.tpp;
   const int D = p.D;
 
-  // ---- this workgroup's share [lo, hi) of all tiles, and the sequence it begins in
-  int64_t lo = 0, hi = 0, share = 0, extra = 0;
-  int b = 0;
-  int64_t base = 0;  // tiles before sequence b
+  // ---- this workgroup's share [lo, hi) of all tiles.  Every wave sums over the
+  // batch by itself (a lane takes `per` sequences in a row), so nothing waits.
+  const int per = (p.B + 63) / 64;
+  Seq held = {0, 0, 0};  // per == 1: lane b's is sequence b
+  int b = 0, base = 0;   // the sequence at hand, the tiles before it
+  int lo = 0, hi = 0, share = 0, extra = 0;
+  bool idle = !a.split;  // a sequence has no tiles
+  // sequence of the batch, the same for every lane
+  auto seq_at = [&](int i) {
+    Seq s;
+    if (per == 1) {
+      s.len = __builtin_amdgcn_readlane(held.len, i);
+      s.fresh = __builtin_amdgcn_readlane(held.fresh, i);
+      s.tiles = __builtin_amdgcn_readlane(held.tiles, i);
+    } else {
+      s = seq_of<SEL>(p, i, tpp);
+      s.len = __builtin_amdgcn_readfirstlane(s.len);
+      s.fresh = __builtin_amdgcn_readfirstlane(s.fresh);
+      s.tiles = __builtin_amdgcn_readfirstlane(s.tiles);
+    }
+    return s;
+  };
+  if (per == 1 && lane < p.B) held = seq_of<SEL>(p, lane, tpp);
   if (a.split) {
-    const int per = (p.B + NT - 1) / NT;
-    const int b0 = min(tid * per, p.B), b1 = min(b0 + per, p.B);
-    int64_t mine = 0;
-    for (int i = b0; i < b1; ++i) mine += (int64_t)tiles_of<SEL>(p, i, tpp) * U;
-    int64_t inc = mine;
-#pragma unroll
-    for (int d = 1; d < 64; d <<= 1) {
-      const int64_t up = __shfl_up(inc, d);
-      if (lane >= d) inc += up;
-    }
-    if (lane == 63) s_wsum[wave] = inc;
-    __syncthreads();
-    int64_t total = 0, before = 0;
-#pragma unroll
-    for (int w = 0; w < NW; ++w) {
-      if (w < wave) before += s_wsum[w];
-      total += s_wsum[w];
-    }
-    const int64_t ex = before + inc - mine;
-    const int64_t want = total / kMinTiles;
-    const int n = want < 1 ? 1 : want < nwg ? (int)want : nwg;
-    if (total > 0 && wg < n) {
-      share = total / n;
-      extra = total - share * n;
-      lo = wg * share + (wg < extra ? wg : extra);
-      hi = lo + share + (wg < extra ? 1 : 0);
-      if (lo >= ex && lo < ex + mine) {
-        int64_t at = ex;
-        for (int i = b0; i < b1; ++i) {
-          const int64_t t = (int64_t)tiles_of<SEL>(p, i, tpp) * U;
-          if (lo < at + t) {
-            s_b = i;
-            s_at[0] = at;
-            break;
-          }
-          at += t;
-        }
+    const int b0 = min(lane * per, p.B), b1 = min(b0 + per, p.B);
+    int tiles = 0, busy = 0;
+    if (per == 1) {
+      tiles = held.tiles;
+      busy = tiles > 0;
+    } else {
+      for (int i = b0; i < b1; ++i) {
+        const int t = seq_of<SEL>(p, i, tpp).tiles;
+        tiles += t;
+        busy += t > 0;
       }
     }
-    __syncthreads();
-    if (lo < hi) {
-      b = __builtin_amdgcn_readfirstlane(s_b);
-      base = s_at[0];
+    int inc = tiles, all = busy;
+#pragma unroll
+    for (int d = 1; d < 64; d <<= 1) {
+      const int up = __shfl_up(inc, d), more = __shfl_xor(all, d);
+      if (lane >= d) inc += up;
+      all += more;
+    }
+    all = __builtin_amdgcn_readfirstlane(all);
+    idle = all < p.B;
+    const int total = __builtin_amdgcn_readlane(inc, 63) * U;
+    // as many shares as workgroups, but of kMinTiles tiles at least, or a unit each
+    const int n = min(nwg, max(total / kMinTiles, all * U));
+    if (wg < n) {
+      share = total / n;
+      extra = total - share * n;
+      lo = wg * share + min(wg, extra);
+      hi = lo + share + (wg < extra ? 1 : 0);
+      // units of kWhole tiles or fewer are not split: a share begins (and ends)
+      // behind the unit its border falls into
+      auto border = [&](int x, int& seq, int& before) {
+        if (x >= total) return total;
+        const uint64_t in = __builtin_amdgcn_ballot_w64((inc - tiles) * U <= x && x < inc * U);
+        const int at = (int)__builtin_ctzll(in);
+        before = __builtin_amdgcn_readlane(inc - tiles, at) * U;
+        seq = at * per;
+        Seq s = seq_at(seq);
+        while (x >= before + s.tiles * U) {
+          before += s.tiles * U;
+          s = seq_at(++seq);
+        }
+        if (s.tiles > kWhole) return x;
+        const int i = (x - before + s.tiles - 1) / s.tiles;
+        return before + i * s.tiles;
+      };
+      int seq = 0, before = 0;
+      hi = border(hi, seq, before);
+      lo = border(lo, b, base);
     }
   }
-  // the workgroup that holds tile x
-  auto wg_of = [&](int64_t x) {
-    const int64_t edge = (share + 1) * extra;
-    return (int)(x < edge ? x / (share + 1) : extra + (x - edge) / share);
+  // the workgroup that holds tile x of a unit that may be split
+  auto wg_of = [&](int x) {
+    const int edge = (share + 1) * extra;
+    return x < edge ? x / (share + 1) : extra + (x - edge) / share;
   };
 
   // ---- constant per-lane offsets
@@ -229,54 +272,55 @@ __global__ __launch_bounds__(pg_waves(DK * sizeof(T)) * 64, 1) void paged_attn(P
   const float cmul = p.c;
   auto weight = [](float m, float mx) { return m == -INFINITY ? 0.f : fast_exp2(m - mx); };
 
-  int unit = a.split ? 0 : wg;  // whole units: the one to do next
-  int64_t x = lo;
+  int unit = wg;  // whole units: the one to do next
+  int x = lo;
   bool more = a.split ? x < hi : unit < p.B * U;
   while (more) {
     // ---- the next segment: tiles [ta, tb) of unit (b, i), one of `parts`, the part-th
-    int nt, i, ta = 0, tb, parts = 1, part = 0, w0 = 0;
+    Seq seq;
+    int i, ta = 0, tb, parts = 1, part = 0, w0 = 0;
     if (a.split) {
-      nt = __builtin_amdgcn_readfirstlane(tiles_of<SEL>(p, b, tpp));
-      while (x >= base + (int64_t)nt * U) {
-        base += (int64_t)nt * U;
-        ++b;
-        nt = __builtin_amdgcn_readfirstlane(tiles_of<SEL>(p, b, tpp));
+      seq = seq_at(b);
+      while (x >= base + seq.tiles * U) {
+        base += seq.tiles * U;
+        seq = seq_at(++b);
       }
-      i = (int)((x - base) / nt);
-      const int64_t u0 = base + (int64_t)i * nt, u1 = u0 + nt;
-      ta = (int)(x - u0);
-      tb = (int)((hi < u1 ? hi : u1) - u0);
-      w0 = ta == 0 ? wg : wg_of(u0);
-      parts = (tb == nt ? wg : wg_of(u1 - 1)) - w0 + 1;
-      part = wg - w0;
+      i = (x - base) / seq.tiles;
+      const int u0 = base + i * seq.tiles, u1 = u0 + seq.tiles;
+      ta = x - u0;
+      tb = min(hi, u1) - u0;
+      if (ta > 0 || tb < seq.tiles) {
+        w0 = ta == 0 ? wg : wg_of(u0);
+        parts = (tb == seq.tiles ? wg : wg_of(u1 - 1)) - w0 + 1;
+        part = wg - w0;
+      }
       x = u0 + tb;
       more = x < hi;
     } else {
       b = unit / U;
       i = unit - b * U;
-      nt = __builtin_amdgcn_readfirstlane(tiles_of<SEL>(p, b, tpp));
-      tb = nt;
+      seq = seq_at(b);
+      tb = seq.tiles;
       unit += nwg;
       more = unit < p.B * U;
-      if (nt == 0) continue;
+      if (tb == 0) continue;
     }
-    b = __builtin_amdgcn_readfirstlane(b);
-    const int hk = __builtin_amdgcn_readfirstlane(i / RBLK);
-    const int row0 = (i - hk * RBLK) * kRows;
+    const int len = seq.len, fresh = seq.fresh;
+    const int hk = a.blocks == 1 ? i : i / a.blocks;
+    const int row0 = (i - hk * a.blocks) * kRows;
     const int R = min(kRows, rows_all - row0);
-    const int len = __builtin_amdgcn_readfirstlane(seq_len_held(p.map, b));
-    const int fresh = __builtin_amdgcn_readfirstlane(seq_new(p.map, b, p.S, len));
     const int mine = tb - ta > wave ? (tb - ta - wave + NW - 1) / NW : 0;  // tiles of this wave
 
     // offset (elements) of this unit's row r in a [B, H, S, D] tensor
     auto row_of = [&](int r, int64_t h_str, int64_t s_str) {
+      if (p.S == 1) return (int64_t)(hk * G + row0 + r) * h_str;
       const int hr = (row0 + r) / p.S;
       return (int64_t)(hk * G + hr) * h_str + (int64_t)(row0 + r - hr * p.S) * s_str;
     };
     // row c sees the keys before `limit`; every row those before `sure`
     int limit = 0;
     if (c < R) {
-      const int col = (row0 + c) % p.S;
+      const int col = p.S == 1 ? 0 : (row0 + c) % p.S;
       limit = col < fresh ? len - fresh + col + 1 : 0;
     }
     const int sure = p.S == 1 ? len : 0;
@@ -292,38 +336,51 @@ __global__ __launch_bounds__(pg_waves(DK * sizeof(T)) * 64, 1) void paged_attn(P
       }
     }
 
-    // ---- pages of this wave's tiles [64 k, 64 k + 64): lane l those of tile 64 k + l
-    int my_page = 0, my_pos = 0;  // page number (-1: nothing to read), position of the tile's first key
+    // ---- what this wave's tiles [64 k, 64 k + 64) read, lane l's that of tile
+    // 64 k + l: the page's address at the tile's first slot and the bytes from
+    // there that hold keys (K and V), the position of the first key and the
+    // tile's slots
+    uint32_t ka[2], va[2];
+    int kn = 0, vn = 0, pos0 = 0, slots0 = 0;
     bool bad = false;
     auto fetch = [&](int k) {
       const int j = 64 * k + lane, t = ta + wave + NW * j;
-      my_page = -1;
-      my_pos = 0;
+      int page = -1;
+      kn = vn = pos0 = slots0 = 0;
+      int slot = 0;
       if (j < mine) {
-        const int e = t / tpp, sub = t - e * tpp;
+        const int e = tpp == 1 ? t : t / tpp;
+        slot = (t - e * tpp) * kTile;
         const int col = SEL ? p.selected[((int64_t)b * p.Hkv + hk) * p.n_selected + e] : e;
         if (col >= 0) {
-          my_page = (int64_t)col * ps < len ? page_at(p.map, b, col) : -1;
-          my_pos = col * ps + sub * kTile;
-          bad |= my_page < 0;
+          page = col <= (len - 1) / ps ? page_at(p.map, b, col) : -1;
+          bad |= page < 0;
+          pos0 = page < 0 ? 0 : col * ps + slot;
+          slots0 = page < 0 ? 0 : min(min(kTile, ps - slot), max(len - pos0, 0));
         }
       }
+      if (slots0 > 0) {
+        kn = (slots0 - 1) * ks_b + D * ES;
+        vn = (slots0 - 1) * vs_b + D * ES;
+      }
+      const uint64_t kb = (uint64_t)((const char*)p.k + (max(page, 0) * p.kp_p + hk * p.kp_h + slot * p.kp_s) * ES);
+      const uint64_t vb = (uint64_t)((const char*)p.v + (max(page, 0) * p.vp_p + hk * p.vp_h + slot * p.vp_s) * ES);
+      ka[0] = (uint32_t)kb;
+      ka[1] = (uint32_t)(kb >> 32) & 0xffffu;
+      va[0] = (uint32_t)vb;
+      va[1] = (uint32_t)(vb >> 32) & 0xffffu;
     };
+    auto at_lane = [](uint32_t v, int l) { return (uint32_t)__builtin_amdgcn_readlane((int)v, l); };
     // this wave's tile j into stage j % NS
     auto issue = [&](int j) {
-      const int page = __builtin_amdgcn_readlane(my_page, j & 63);
-      const int pos = __builtin_amdgcn_readlane(my_pos, j & 63);
-      const int slot = pos % ps;
-      const int n = page < 0 ? 0 : min(min(kTile, ps - slot), len - pos);  // valid slots (<= 0: none)
-      const char* kb = (const char*)p.k + ((int64_t)max(page, 0) * p.kp_p + hk * p.kp_h + slot * p.kp_s) * ES;
-      const char* vb = (const char*)p.v + ((int64_t)max(page, 0) * p.vp_p + hk * p.vp_h + slot * p.vp_s) * ES;
-      const u32x4 krw = uniform_rsrc_words(kb, n > 0 ? (int64_t)(n - 1) * ks_b + D * ES : 0);
-      const u32x4 vrw = uniform_rsrc_words(vb, n > 0 ? (int64_t)(n - 1) * vs_b + D * ES : 0);
+      const int l = j & 63;
+      const u32x4 krw = {at_lane(ka[0], l), at_lane(ka[1], l), at_lane(kn, l), 0x00020000u};
+      const u32x4 vrw = {at_lane(va[0], l), at_lane(va[1], l), at_lane(vn, l), 0x00020000u};
       const uint32_t st = ring + (uint32_t)((j % NS) * STAGE);
 #pragma unroll
-      for (int q = 0; q < IB; ++q) lds_dma16(krw, st + 1024 * q, kdo[q], 0);
+      for (int q = 0; q < IB; ++q) lds_dma16_fresh(krw, st + 1024 * q, kdo[q]);
 #pragma unroll
-      for (int q = 0; q < IB; ++q) lds_dma16(vrw, st + BLK + 1024 * q, vdo[q], 0);
+      for (int q = 0; q < IB; ++q) lds_dma16_fresh(vrw, st + BLK + 1024 * q, vdo[q]);
     };
 
     f32x4 oacc[NDB];
@@ -332,15 +389,15 @@ __global__ __launch_bounds__(pg_waves(DK * sizeof(T)) * 64, 1) void paged_attn(P
     float m_run = -INFINITY, l_run = 0.f;
 
     fetch(0);
-    // (pages, positions) of the tile at hand: the lanes move on to the next 64
-    // tiles when the first tile past them is issued, up to NS tiles ahead
-    int pos_q[NS];
+    // (position, slots) of the tiles in flight: the lanes move on to the next 64
+    // tiles when the first of those is issued, up to NS tiles ahead
+    int pos_q[NS], slots_q[NS];
 #pragma unroll
     for (int j = 0; j < NS; ++j) {
-      pos_q[j] = 0;
+      pos_q[j] = slots_q[j] = 0;
       if (j < mine) {
-        pos_q[j] = __builtin_amdgcn_readlane(my_pos, j);
-        if (__builtin_amdgcn_readlane(my_page, j) < 0) pos_q[j] = -1;
+        pos_q[j] = __builtin_amdgcn_readlane(pos0, j);
+        slots_q[j] = __builtin_amdgcn_readlane(slots0, j);
         issue(j);
       }
     }
@@ -352,9 +409,12 @@ __global__ __launch_bounds__(pg_waves(DK * sizeof(T)) * 64, 1) void paged_attn(P
       else if (behind == 1) wait_vmcnt<IPT <= 63 ? IPT : 63>();
       else wait_vmcnt<0>();
       const unsigned char* st = lds + (wave * NS + j % NS) * STAGE;
-      const int pos = pos_q[0];
+      const int pos = pos_q[0], slots = slots_q[0];
 #pragma unroll
-      for (int q = 0; q + 1 < NS; ++q) pos_q[q] = pos_q[q + 1];
+      for (int q = 0; q + 1 < NS; ++q) {
+        pos_q[q] = pos_q[q + 1];
+        slots_q[q] = slots_q[q + 1];
+      }
 
       f32x4 s = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
@@ -371,11 +431,10 @@ __global__ __launch_bounds__(pg_waves(DK * sizeof(T)) * 64, 1) void paged_attn(P
       float xs[4];
 #pragma unroll
       for (int e = 0; e < 4; ++e) xs[e] = s[e] * cmul;
-      const int slots = min(kTile, ps - pos % ps);
-      if (pos < 0 || pos + kTile > sure || slots < kTile) {
+      if (slots < kTile || pos + kTile > sure) {
 #pragma unroll
         for (int e = 0; e < 4; ++e)
-          if (pos < 0 || pos + 4 * g + e >= limit || 4 * g + e >= slots) xs[e] = -INFINITY;
+          if (4 * g + e >= slots || pos + 4 * g + e >= limit) xs[e] = -INFINITY;
       }
       float mt = fmaxf(fmaxf(xs[0], xs[1]), fmaxf(xs[2], xs[3]));
       mt = fmaxf(mt, xor_f(mt, 16));
@@ -392,9 +451,9 @@ __global__ __launch_bounds__(pg_waves(DK * sizeof(T)) * 64, 1) void paged_attn(P
       float pe[4];
 #pragma unroll
       for (int e = 0; e < 4; ++e) pe[e] = fast_exp2(xs[e] - m_sub);
+      l_run += (pe[0] + pe[1]) + (pe[2] + pe[3]);
       const unsigned char* vs = st + BLK;
       if constexpr (F32) {
-        l_run += (pe[0] + pe[1]) + (pe[2] + pe[3]);
         // 64 columns at a time: MFMA j takes columns 4 m + j (a lane's 16-byte
         // read is one slot's chunk, an element for each of the four)
 #pragma unroll
@@ -409,10 +468,11 @@ __global__ __launch_bounds__(pg_waves(DK * sizeof(T)) * 64, 1) void paged_attn(P
           }
         }
       } else {
-        u32x2 pb;
+        u32x2 pb, pl;
         pb[0] = Mma<T>::pack(pe[0], pe[1]);
         pb[1] = Mma<T>::pack(pe[2], pe[3]);
-        l_run = Mma<T>::sum2(pb[1], Mma<T>::sum2(pb[0], l_run));
+        pl[0] = Mma<T>::rest(pb[0], pe[0], pe[1]);
+        pl[1] = Mma<T>::rest(pb[1], pe[2], pe[3]);
         // 16 lanes of group g read slots 4g .. 4g+3 x 16 columns, transposed:
         // lane c receives column 16 db + c of the four
         const int r = 4 * g + (c >> 2), ch = (c & 3) >> 1;
@@ -422,12 +482,13 @@ __global__ __launch_bounds__(pg_waves(DK * sizeof(T)) * 64, 1) void paged_attn(P
           const unsigned char* at = vs + r * RB + 16 * pg_swz(r, 2 * db + ch, NC) + 8 * (c & 1);
           const i16x4p v = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_i16x4*)at);
           oacc[db] = Mma<T>::pv(__builtin_bit_cast(u32x2, v), pb, oacc[db]);
+          oacc[db] = Mma<T>::pv(__builtin_bit_cast(u32x2, v), pl, oacc[db]);
         }
       }
       if (j + NS < mine) {
         if (((j + NS) & 63) == 0) fetch((j + NS) >> 6);
-        pos_q[NS - 1] = __builtin_amdgcn_readlane(my_pos, (j + NS) & 63);
-        if (__builtin_amdgcn_readlane(my_page, (j + NS) & 63) < 0) pos_q[NS - 1] = -1;
+        pos_q[NS - 1] = __builtin_amdgcn_readlane(pos0, (j + NS) & 63);
+        slots_q[NS - 1] = __builtin_amdgcn_readlane(slots0, (j + NS) & 63);
         // this stage's LDS reads have returned before its next tile's loads go out
         asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
         issue(j + NS);
@@ -594,10 +655,10 @@ __global__ __launch_bounds__(pg_waves(DK * sizeof(T)) * 64, 1) void paged_attn(P
   }
 
   // ---- places nothing was read for: zeros, NaN where the sequence is longer than its table row
-  for (int bb = wg; bb < p.B; bb += nwg) {
-    if (tiles_of<SEL>(p, bb, tpp) > 0) continue;
-    const int len = seq_len_held(p.map, bb);
-    const bool err = len > p.map.width * ps && seq_new(p.map, bb, p.S, len) > 0;
+  for (int bb = idle ? wg : p.B; bb < p.B; bb += nwg) {
+    const Seq seq = seq_of<SEL>(p, bb, tpp);
+    if (seq.tiles > 0) continue;
+    const bool err = seq.len > p.map.width * ps && seq.fresh > 0;
     const uint32_t w = err ? (F32 ? 0x7fc00000u : 0x7fff7fffu) : 0u;
     const int nc = D * ES / 16;
     for (int u = tid; u < p.H * p.S * nc; u += NT) {
@@ -622,8 +683,8 @@ int workgroups(int dtype, int B, int H, int Hkv, int S, int D, int page_size, in
   const int64_t units = (int64_t)B * Hkv * ((H / Hkv * S + kRows - 1) / kRows);
   const int64_t cols = n_selected > 0 ? n_selected : width;
   const int64_t tiles = units * cols * ((page_size + kTile - 1) / kTile);
-  const int64_t most = (tiles + kMinTiles - 1) / kMinTiles;
-  return most < 1 ? 1 : most < n ? (int)most : n;
+  const int64_t most = tiles / kMinTiles > units ? tiles / kMinTiles : units;
+  return most < n ? (int)most : n;
 }
 
 template <typename T, int DK>
@@ -650,7 +711,10 @@ hipError_t launch16(const PagedAttnParams& p, const Plan& a, int wgs, hipStream_
 
 size_t paged_attn_workspace(int dtype, int B, int H, int Hkv, int S, int D, int page_size, int width, int n_selected) {
   const int n = workgroups(dtype, B, H, Hkv, S, D, page_size, width, n_selected);
-  if (n <= 1) return 0;
+  // tiles are counted in 32 bits: a table for more is read in whole units
+  const int64_t cols = n_selected > 0 ? n_selected : width;
+  const int64_t units = (int64_t)B * Hkv * ((H / Hkv * S + kRows - 1) / kRows);
+  if (n <= 1 || units * cols * ((page_size + kTile - 1) / kTile) > INT32_MAX - kMaxWgs) return 0;
   return kExchangeCounterBytes + (size_t)n * 2 * kRows * (bucket(dtype, D) / 4 + 1) * sizeof(f32x4);
 }
 
@@ -658,7 +722,8 @@ hipError_t launch_paged_attn(const PagedAttnParams& p, int dtype, hipStream_t s)
   const int ps = p.map.page_size;
   const size_t need = paged_attn_workspace(dtype, p.B, p.H, p.Hkv, p.S, p.D, ps, p.map.width, p.n_selected);
   int wgs = workgroups(dtype, p.B, p.H, p.Hkv, p.S, p.D, ps, p.map.width, p.n_selected);
-  Plan a = {nullptr, nullptr, 0};
+  const int G = p.H / p.Hkv, blocks = (G * p.S + kRows - 1) / kRows, tpp = (ps + kTile - 1) / kTile;
+  Plan a = {nullptr, nullptr, 0, G, blocks, p.Hkv * blocks, tpp};
   if (need > 0 && p.workspace && p.workspace_bytes >= need) {
     a.cnt = (int*)p.workspace;
     a.ws = (f32x4*)((char*)p.workspace + kExchangeCounterBytes);
