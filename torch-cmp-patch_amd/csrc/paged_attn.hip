@@ -29,6 +29,8 @@
 //    in the workspace and counts itself in, and the last one joins the parts in
 //    their order and puts the counter back to zero.  Nobody waits for another
 //    workgroup.
+#include <string.h>
+
 #include "paged_common.h"
 
 namespace cmpext3 {
@@ -77,6 +79,7 @@ constexpr int kRows = 16;        // query rows of a unit at most
 constexpr int kTile = 16;        // slots of a tile
 constexpr int kMaxWgs = 1024;    // workgroups of a launch at most (counters: one each)
 constexpr int kMinTiles = 16;    // tiles of a workgroup's share at least
+constexpr int kSetup = 6;        // what a unit costs beside its tiles, in tiles
 constexpr int kWhole = 32;       // tiles of a unit that is never split
 constexpr int kMergeLoads = 8;   // loads of one merging thread in flight together
 
@@ -104,15 +107,43 @@ __device__ __forceinline__ void lds_dma16_fresh(const u32x4& rs, uint32_t lds_by
   asm volatile("s_nop 4\n\tbuffer_load_dwordx4 %0, %1, 0 offen lds" ::"v"(voff), "s"(rs), "{m0}"(lds_byte) : "memory");
 }
 
-struct Plan {
+// n / d for 0 <= n < 2^31 as a product: s = ceil(log2 d), m = floor(2^(31+s) / d)
+// + 1 exceeds the quotient's scale by less than 2^s / 2^(31+s), too little to
+// reach the next whole number.
+struct Div {
+  uint32_t m;
+  int s;
+};
+__device__ __forceinline__ int quot(int n, uint32_t m, int s) { return (int)(__umulhi((uint32_t)n << 1, m) >> s); }
+
+struct AttnArgs {
+  const int32_t *lens, *news, *table, *selected;
+  int64_t t_str;
+  int B, S, U, cap;        // U: units of a sequence; cap: keys a table row holds
+  int nsel, width, ps, tpp;  // tpp: tiles per page
+  Div by_ps, by_tpp, by_blocks, by_s;
+  int split, exact;        // split 0: whole units, dealt out in turn; exact: pages are whole tiles
+  int G, blocks, rows, num_pages;  // query heads per K/V head, row blocks and rows of a K/V head
+  const char *k, *v;
+  int64_t kp_p, kp_h, vp_p, vp_h;  // bytes
+  int ks_b, vs_b, row_b, D;        // bytes of a slot's stride, of a row
+  const void* q;
+  int64_t q_b, q_h, q_s;
+  void* o;
+  int64_t o_b, o_h, o_s;
+  float c;
+  uint32_t q_sign;
   f32x4* ws;  // parts: [workgroup][first or last segment][row] (DK / 4 + 1) float4: O, then (m, l, 0, 0)
   int* cnt;   // a counter for the unit that a workgroup's last segment begins
-  int split;  // 0: whole units, dealt out in turn
-  int group;  // query heads per K/V head
-  int blocks; // row blocks per (sequence, K/V head)
-  int units;  // of a sequence
-  int tpp;    // tiles per page
 };
+typedef const __attribute__((address_space(4))) AttnArgs* ArgsPtr;
+// The arguments, read anew from here on: a phase of the kernel loads those it
+// uses, and none has to stay in (or spill from) scalar registers between
+// phases.
+__device__ __forceinline__ ArgsPtr anew(ArgsPtr p) {
+  asm volatile("" : "+s"(p));
+  return p;
+}
 
 // A sequence as the launch sees it.
 struct Seq {
@@ -120,22 +151,35 @@ struct Seq {
   int tiles;       // 0: nothing of it is read (no tokens, no new ones, or longer than its table row)
 };
 template <bool SEL>
-__device__ __forceinline__ Seq seq_of(const PagedAttnParams& p, int b, int tpp) {
+__device__ __forceinline__ Seq seq_of(ArgsPtr p, int b) {
   Seq s;
-  const int ps = p.map.page_size;
-  s.len = seq_len_held(p.map, b);
-  s.fresh = seq_new(p.map, b, p.S, s.len);
-  if (s.fresh == 0 || s.len > p.map.width * ps) s.tiles = 0;
-  else if (SEL) s.tiles = p.n_selected * tpp;
-  else if (tpp * kTile == ps) s.tiles = (s.len + kTile - 1) / kTile;
-  else s.tiles = s.len / ps * tpp + (s.len % ps + kTile - 1) / kTile;
+  s.len = min(max(p->lens[b], 0), p->cap + 1);
+  s.fresh = min(p->news ? min(max(p->news[b], 0), p->S) : p->S, s.len);
+  if (s.fresh == 0 || s.len > p->cap) s.tiles = 0;
+  else if (SEL) s.tiles = p->nsel * p->tpp;
+  else if (p->exact) s.tiles = (s.len + kTile - 1) / kTile;
+  else {
+    const int full = quot(s.len, p->by_ps.m, p->by_ps.s);
+    s.tiles = full * p->tpp + (s.len - full * p->ps + kTile - 1) / kTile;
+  }
   return s;
+}
+
+// Sum over the lanes up to this one.
+__device__ __forceinline__ int wave_scan(int v) {
+  v += __builtin_amdgcn_update_dpp(0, v, 0x111, 0xf, 0xf, false);  // row_shr 1, 2, 4, 8
+  v += __builtin_amdgcn_update_dpp(0, v, 0x112, 0xf, 0xf, false);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x114, 0xf, 0xf, false);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x118, 0xf, 0xf, false);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x142, 0xa, 0xf, false);  // row_bcast 15, 31
+  v += __builtin_amdgcn_update_dpp(0, v, 0x143, 0xc, 0xf, false);
+  return v;
 }
 
 __device__ __forceinline__ float xor_f(float x, int m) { return __shfl_xor(x, m); }
 
 template <typename T, int DK, bool SEL>
-__global__ __launch_bounds__(pg_waves(DK * sizeof(T)) * 64, 1) void paged_attn(PagedAttnParams p, Plan a) {
+__global__ __launch_bounds__(pg_waves(DK * sizeof(T)) * 64, 1) void paged_attn(AttnArgs) {
   constexpr bool F32 = sizeof(T) == 4;
   constexpr int ES = sizeof(T);
   constexpr int RB = DK * ES;           // bytes of a K/V row in LDS
@@ -160,104 +204,80 @@ __global__ __launch_bounds__(pg_waves(DK * sizeof(T)) * 64, 1) void paged_attn(P
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int wg = block_x(), nwg = (int)gridDim.x;
   const int c = lane & 15, g = lane >> 4;
-  const int G = a.group, rows_all = G * p.S, U = a.units;
-  const int ps = p.map.page_size, tpp = a.tpp;
-  const int D = p.D;
+  const ArgsPtr args = (ArgsPtr)__builtin_amdgcn_kernarg_segment_ptr();
 
-  // ---- this workgroup's share [lo, hi) of all tiles.  Every wave sums over the
-  // batch by itself (a lane takes `per` sequences in a row), so nothing waits.
-  const int per = (p.B + 63) / 64;
-  Seq held = {0, 0, 0};  // per == 1: lane b's is sequence b
-  int b = 0, base = 0;   // the sequence at hand, the tiles before it
-  int lo = 0, hi = 0, share = 0, extra = 0;
-  bool idle = !a.split;  // a sequence has no tiles
-  // sequence of the batch, the same for every lane
+  // ---- this workgroup's share [lo, hi) of all units, counted in tiles (plus
+  // kSetup for each unit's own cost).  Every wave sums over the batch by itself
+  // (a lane takes `per` sequences in a row), so nothing waits.
+  int b = 0, base = 0;  // the sequence at hand, what lies before it
+  int x = 0, hi = 0, share = 1;
+  bool idle = true;     // a sequence has no tiles
+  Seq held = {0, 0, 0};  // B <= 64: lane b's is sequence b
+  auto weight_of = [](int tiles) { return tiles > 0 ? tiles + kSetup : 0; };
+  // sequence i of the batch, the same for every lane
   auto seq_at = [&](int i) {
-    Seq s;
-    if (per == 1) {
-      s.len = __builtin_amdgcn_readlane(held.len, i);
-      s.fresh = __builtin_amdgcn_readlane(held.fresh, i);
-      s.tiles = __builtin_amdgcn_readlane(held.tiles, i);
-    } else {
-      s = seq_of<SEL>(p, i, tpp);
-      s.len = __builtin_amdgcn_readfirstlane(s.len);
-      s.fresh = __builtin_amdgcn_readfirstlane(s.fresh);
-      s.tiles = __builtin_amdgcn_readfirstlane(s.tiles);
+    Seq s = held;
+    const ArgsPtr p = anew(args);
+    if (p->B > 64) {
+      s = seq_of<SEL>(p, i);
+      i = 0;
     }
+    s.len = __builtin_amdgcn_readlane(s.len, i);
+    s.fresh = __builtin_amdgcn_readlane(s.fresh, i);
+    s.tiles = __builtin_amdgcn_readlane(s.tiles, i);
     return s;
   };
-  if (per == 1 && lane < p.B) held = seq_of<SEL>(p, lane, tpp);
-  if (a.split) {
-    const int b0 = min(lane * per, p.B), b1 = min(b0 + per, p.B);
-    int tiles = 0, busy = 0;
-    if (per == 1) {
-      tiles = held.tiles;
-      busy = tiles > 0;
-    } else {
-      for (int i = b0; i < b1; ++i) {
-        const int t = seq_of<SEL>(p, i, tpp).tiles;
-        tiles += t;
-        busy += t > 0;
+  {
+    const ArgsPtr p = anew(args);
+    const int B = p->B, U = p->U, per = (B + 63) >> 6;
+    int sum = 0, busy = 0;
+    for (int k = 0, i = lane * per; k < per; ++k, ++i) {
+      if (i < B) {
+        held = seq_of<SEL>(p, i);
+        sum += weight_of(held.tiles);
+        busy += held.tiles > 0;
       }
     }
-    int inc = tiles, all = busy;
-#pragma unroll
-    for (int d = 1; d < 64; d <<= 1) {
-      const int up = __shfl_up(inc, d), more = __shfl_xor(all, d);
-      if (lane >= d) inc += up;
-      all += more;
-    }
-    all = __builtin_amdgcn_readfirstlane(all);
-    idle = all < p.B;
-    const int total = __builtin_amdgcn_readlane(inc, 63) * U;
-    // as many shares as workgroups, but of kMinTiles tiles at least, or a unit each
-    const int n = min(nwg, max(total / kMinTiles, all * U));
-    if (wg < n) {
-      share = total / n;
-      extra = total - share * n;
-      lo = wg * share + min(wg, extra);
-      hi = lo + share + (wg < extra ? 1 : 0);
-      // units of kWhole tiles or fewer are not split: a share begins (and ends)
-      // behind the unit its border falls into
-      auto border = [&](int x, int& seq, int& before) {
-        if (x >= total) return total;
-        const uint64_t in = __builtin_amdgcn_ballot_w64((inc - tiles) * U <= x && x < inc * U);
-        const int at = (int)__builtin_ctzll(in);
-        before = __builtin_amdgcn_readlane(inc - tiles, at) * U;
-        seq = at * per;
-        Seq s = seq_at(seq);
-        while (x >= before + s.tiles * U) {
-          before += s.tiles * U;
-          s = seq_at(++seq);
+    if (p->split) {
+      const int inc = wave_scan(sum);
+      const int total = __builtin_amdgcn_readlane(inc, 63) * U;
+      const int all = __builtin_amdgcn_readlane(wave_scan(busy), 63);
+      idle = all < B;
+      // as many shares as workgroups, but of kMinTiles at least, or a unit each
+      const int n = min(nwg, max(total / kMinTiles, all * U));
+      if (wg < n) {
+        share = (int)(((uint32_t)total + (uint32_t)n - 1u) / (uint32_t)n);
+        x = wg * share;
+        hi = min(x + share, total);
+        const uint64_t in = __builtin_amdgcn_ballot_w64((inc - sum) * U <= x && x < inc * U);
+        if (x < hi) {
+          const int at = (int)__builtin_ctzll(in);
+          base = __builtin_amdgcn_readlane(inc - sum, at) * U;
+          b = at * per;
         }
-        if (s.tiles > kWhole) return x;
-        const int i = (x - before + s.tiles - 1) / s.tiles;
-        return before + i * s.tiles;
-      };
-      int seq = 0, before = 0;
-      hi = border(hi, seq, before);
-      lo = border(lo, b, base);
+      }
+    } else {
+      x = wg;
+      hi = B * U;
     }
   }
-  // the workgroup that holds tile x of a unit that may be split
-  auto wg_of = [&](int x) {
-    const int edge = (share + 1) * extra;
-    return x < edge ? x / (share + 1) : extra + (x - edge) / share;
-  };
 
   // ---- constant per-lane offsets
   // DMA: instruction i writes LDS bytes [1024 i, 1024 i + 1024); lane l's 16
   // bytes land at 1024 i + 16 l: row r, physical chunk pc, holding logical
   // chunk pg_swz(r, pc) of slot r.  Chunks past the head dim read zeros.
-  const int ks_b = (int)p.kp_s * ES, vs_b = (int)p.vp_s * ES;
   int kdo[IB], vdo[IB];
+  {
+    const ArgsPtr p = anew(args);
+    const int ks_b = p->ks_b, vs_b = p->vs_b, row_b = p->row_b;
 #pragma unroll
-  for (int i = 0; i < IB; ++i) {
-    const int pos = 1024 * i + 16 * lane;
-    const int r = pos / RB, lc = pg_swz(r, (pos - r * RB) / 16, NC);
-    const bool in = 16 * lc < D * ES;
-    kdo[i] = in ? r * ks_b + 16 * lc : (int)0x80000000u;
-    vdo[i] = in ? r * vs_b + 16 * lc : (int)0x80000000u;
+    for (int i = 0; i < IB; ++i) {
+      const int pos = 1024 * i + 16 * lane;
+      const int r = pos / RB, lc = pg_swz(r, (pos - r * RB) / 16, NC);
+      const bool in = 16 * lc < row_b;
+      kdo[i] = in ? r * ks_b + 16 * lc : (int)0x80000000u;
+      vdo[i] = in ? r * vs_b + 16 * lc : (int)0x80000000u;
+    }
   }
   int kro[KS];
 #pragma unroll
@@ -269,70 +289,76 @@ __global__ __launch_bounds__(pg_waves(DK * sizeof(T)) * 64, 1) void paged_attn(P
   float* const mo = (float*)lds;
   float* const mm = mo + NW * kRows * MOS;
   float* const ml = mm + NW * kRows;
-  const float cmul = p.c;
   auto weight = [](float m, float mx) { return m == -INFINITY ? 0.f : fast_exp2(m - mx); };
 
-  int unit = wg;  // whole units: the one to do next
-  int x = lo;
-  bool more = a.split ? x < hi : unit < p.B * U;
-  while (more) {
+  while (x < hi) {
     // ---- the next segment: tiles [ta, tb) of unit (b, i), one of `parts`, the part-th
     Seq seq;
     int i, ta = 0, tb, parts = 1, part = 0, w0 = 0;
-    if (a.split) {
+    const ArgsPtr p = anew(args);
+    if (p->split) {
+      const int U = p->U;
       seq = seq_at(b);
-      while (x >= base + seq.tiles * U) {
-        base += seq.tiles * U;
+      int w = weight_of(seq.tiles);
+      while (x >= base + w * U) {
+        base += w * U;
         seq = seq_at(++b);
+        w = weight_of(seq.tiles);
       }
-      i = (x - base) / seq.tiles;
-      const int u0 = base + i * seq.tiles, u1 = u0 + seq.tiles;
-      ta = x - u0;
-      tb = min(hi, u1) - u0;
-      if (ta > 0 || tb < seq.tiles) {
-        w0 = ta == 0 ? wg : wg_of(u0);
-        parts = (tb == seq.tiles ? wg : wg_of(u1 - 1)) - w0 + 1;
+      i = (int)((uint32_t)(x - base) / (uint32_t)w);
+      const int u0 = base + i * w, u1 = u0 + w, x0 = x;
+      x = u1;
+      tb = seq.tiles;
+      if (tb <= kWhole) {  // never split: its first workgroup's
+        if (x0 > u0) continue;
+      } else if (x0 > u0 || hi < u1) {
+        // the workgroup that holds tile 0 has part 0
+        ta = max(x0 - u0 - kSetup, 0);
+        tb = min(min(hi, u1) - u0 - kSetup, tb);
+        if (tb <= ta) continue;
+        w0 = ta == 0 ? wg : (int)((uint32_t)(u0 + kSetup) / (uint32_t)share);
         part = wg - w0;
+        parts = (tb == seq.tiles ? wg : (int)((uint32_t)(u1 - 1) / (uint32_t)share)) - w0 + 1;
       }
-      x = u0 + tb;
-      more = x < hi;
     } else {
-      b = unit / U;
-      i = unit - b * U;
+      b = x / p->U;
+      i = x - b * p->U;
+      x += nwg;
       seq = seq_at(b);
       tb = seq.tiles;
-      unit += nwg;
-      more = unit < p.B * U;
       if (tb == 0) continue;
     }
-    const int len = seq.len, fresh = seq.fresh;
-    const int hk = a.blocks == 1 ? i : i / a.blocks;
-    const int row0 = (i - hk * a.blocks) * kRows;
-    const int R = min(kRows, rows_all - row0);
+    const int len = seq.len, fresh = seq.fresh, S = p->S;
+    const int hk = quot(i, p->by_blocks.m, p->by_blocks.s);
+    const int row0 = (i - hk * p->blocks) * kRows;
+    const int R = min(kRows, p->rows - row0);
+    const int head0 = hk * p->G;
     const int mine = tb - ta > wave ? (tb - ta - wave + NW - 1) / NW : 0;  // tiles of this wave
 
-    // offset (elements) of this unit's row r in a [B, H, S, D] tensor
-    auto row_of = [&](int r, int64_t h_str, int64_t s_str) {
-      if (p.S == 1) return (int64_t)(hk * G + row0 + r) * h_str;
-      const int hr = (row0 + r) / p.S;
-      return (int64_t)(hk * G + hr) * h_str + (int64_t)(row0 + r - hr * p.S) * s_str;
+    // this unit's row r: query head head0 + h, column r - h S
+    auto head_of = [&](int r, int& col) {
+      const ArgsPtr p = anew(args);
+      const int h = quot(row0 + r, p->by_s.m, p->by_s.s);
+      col = row0 + r - h * p->S;
+      return head0 + h;
     };
     // row c sees the keys before `limit`; every row those before `sure`
     int limit = 0;
-    if (c < R) {
-      const int col = p.S == 1 ? 0 : (row0 + c) % p.S;
-      limit = col < fresh ? len - fresh + col + 1 : 0;
-    }
-    const int sure = p.S == 1 ? len : 0;
-
+    const int sure = S == 1 ? len : 0;
     u32x4 qf[KS];
     {
-      const T* qrow = (const T*)p.q + b * p.q_b + (c < R ? row_of(c, p.q_h, p.q_s) : 0);
+      const ArgsPtr p = anew(args);
+      int col;
+      const int h = head_of(c, col);
+      if (c < R && col < fresh) limit = len - fresh + col + 1;
+      const char* qrow = (const char*)p->q + (b * p->q_b + (c < R ? h * p->q_h + col * p->q_s : 0)) * ES;
+      const uint32_t sg = p->q_sign;
+      const int end = c < R ? p->row_b : 0;
 #pragma unroll
       for (int ks = 0; ks < KS; ++ks) {
-        const int ch = 4 * ks + g;
-        u32x4 w = c < R && ch * 16 < D * ES ? *(const u32x4*)((const char*)qrow + 16 * ch) : (u32x4){0u, 0u, 0u, 0u};
-        qf[ks] = w ^ (u32x4){p.q_sign, p.q_sign, p.q_sign, p.q_sign};
+        const int at = 64 * ks + 16 * g;
+        const u32x4 w = at < end ? *(const u32x4*)(qrow + at) : (u32x4){0u, 0u, 0u, 0u};
+        qf[ks] = w ^ (u32x4){sg, sg, sg, sg};
       }
     }
 
@@ -344,27 +370,33 @@ __global__ __launch_bounds__(pg_waves(DK * sizeof(T)) * 64, 1) void paged_attn(P
     int kn = 0, vn = 0, pos0 = 0, slots0 = 0;
     bool bad = false;
     auto fetch = [&](int k) {
+      const ArgsPtr p = anew(args);
       const int j = 64 * k + lane, t = ta + wave + NW * j;
       int page = -1;
       kn = vn = pos0 = slots0 = 0;
       int slot = 0;
       if (j < mine) {
-        const int e = tpp == 1 ? t : t / tpp;
-        slot = (t - e * tpp) * kTile;
-        const int col = SEL ? p.selected[((int64_t)b * p.Hkv + hk) * p.n_selected + e] : e;
+        const int e = quot(t, p->by_tpp.m, p->by_tpp.s);
+        slot = (t - e * p->tpp) * kTile;
+        const int col = SEL ? p->selected[((int64_t)b * (p->U / p->blocks) + hk) * p->nsel + e] : e;
         if (col >= 0) {
-          page = col <= (len - 1) / ps ? page_at(p.map, b, col) : -1;
-          bad |= page < 0;
-          pos0 = page < 0 ? 0 : col * ps + slot;
-          slots0 = page < 0 ? 0 : min(min(kTile, ps - slot), max(len - pos0, 0));
+          if (!SEL || (int64_t)col * p->ps < len) page = p->table[b * p->t_str + col];
+          if (page < 0 || page >= p->num_pages) {
+            page = -1;
+            bad = true;
+          } else {
+            pos0 = col * p->ps + slot;
+            slots0 = min(min(kTile, p->ps - slot), max(len - pos0, 0));
+          }
         }
       }
+      const int ks_b = p->ks_b, vs_b = p->vs_b;
       if (slots0 > 0) {
-        kn = (slots0 - 1) * ks_b + D * ES;
-        vn = (slots0 - 1) * vs_b + D * ES;
+        kn = (slots0 - 1) * ks_b + p->row_b;
+        vn = (slots0 - 1) * vs_b + p->row_b;
       }
-      const uint64_t kb = (uint64_t)((const char*)p.k + (max(page, 0) * p.kp_p + hk * p.kp_h + slot * p.kp_s) * ES);
-      const uint64_t vb = (uint64_t)((const char*)p.v + (max(page, 0) * p.vp_p + hk * p.vp_h + slot * p.vp_s) * ES);
+      const uint64_t kb = (uint64_t)(p->k + max(page, 0) * p->kp_p + hk * p->kp_h + (int64_t)slot * ks_b);
+      const uint64_t vb = (uint64_t)(p->v + max(page, 0) * p->vp_p + hk * p->vp_h + (int64_t)slot * vs_b);
       ka[0] = (uint32_t)kb;
       ka[1] = (uint32_t)(kb >> 32) & 0xffffu;
       va[0] = (uint32_t)vb;
@@ -387,6 +419,7 @@ __global__ __launch_bounds__(pg_waves(DK * sizeof(T)) * 64, 1) void paged_attn(P
 #pragma unroll
     for (int db = 0; db < NDB; ++db) oacc[db] = (f32x4){0.f, 0.f, 0.f, 0.f};
     float m_run = -INFINITY, l_run = 0.f;
+    const float cmul = anew(args)->c;
 
     fetch(0);
     // (position, slots) of the tiles in flight: the lanes move on to the next 64
@@ -519,11 +552,13 @@ __global__ __launch_bounds__(pg_waves(DK * sizeof(T)) * 64, 1) void paged_attn(P
     lds_barrier();
 
     const int nu = R * DQ;  // (row, 4 columns) vectors of the output
-    T* const og = (T*)p.o + b * p.o_b;
     auto inverse = [](float l) { return l == 0.f ? 0.f : 1.f / l; };
     auto store_out = [&](int r, int k, f32x4 o, float inv) {
-      if (4 * k >= D) return;
-      T* const at = og + row_of(r, p.o_h, p.o_s) + 4 * k;
+      const ArgsPtr p = anew(args);
+      if (4 * k >= p->D) return;
+      int col;
+      const int h = head_of(r, col);
+      T* const at = (T*)p->o + b * p->o_b + h * p->o_h + col * p->o_s + 4 * k;
       if constexpr (F32) {
         *(f32x4*)at = o * inv;
       } else {
@@ -533,9 +568,11 @@ __global__ __launch_bounds__(pg_waves(DK * sizeof(T)) * 64, 1) void paged_attn(P
         *(u32x2*)at = w;
       }
     };
+    const ArgsPtr pe_args = anew(args);
     const __amdgpu_buffer_rsrc_t wsr =
-        uniform_rsrc(parts > 1 ? (const void*)a.ws : (const void*)p.o,
+        uniform_rsrc(parts > 1 ? (const void*)pe_args->ws : (const void*)pe_args->o,
                      parts > 1 ? (int64_t)nwg * 2 * kRows * (DQ + 1) * 16 : 16);
+    int* const cnt = pe_args->cnt;
     // slot of part q's row r: a part that begins the unit is its workgroup's
     // last segment, the others are their workgroups' first
     auto slot = [&](int q, int r, int k) { return ((((w0 + q) * 2 + (q == 0 ? 1 : 0)) * kRows + r) * (DQ + 1) + k) * 16; };
@@ -570,8 +607,8 @@ __global__ __launch_bounds__(pg_waves(DK * sizeof(T)) * 64, 1) void paged_attn(P
       asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
       lds_barrier();  // every wave's stores are done
       if (tid == 0) {
-        const int old = __hip_atomic_fetch_add(a.cnt + w0, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-        if (old == parts - 1) __hip_atomic_store(a.cnt + w0, 0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        const int old = __hip_atomic_fetch_add(cnt + w0, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        if (old == parts - 1) __hip_atomic_store(cnt + w0, 0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
         s_flag = old == parts - 1;
       }
       lds_barrier();
@@ -655,15 +692,16 @@ __global__ __launch_bounds__(pg_waves(DK * sizeof(T)) * 64, 1) void paged_attn(P
   }
 
   // ---- places nothing was read for: zeros, NaN where the sequence is longer than its table row
-  for (int bb = idle ? wg : p.B; bb < p.B; bb += nwg) {
-    const Seq seq = seq_of<SEL>(p, bb, tpp);
+  const ArgsPtr p = anew(args);
+  for (int bb = idle ? wg : p->B; bb < p->B; bb += nwg) {
+    const Seq seq = seq_of<SEL>(p, bb);
     if (seq.tiles > 0) continue;
-    const bool err = seq.len > p.map.width * ps && seq.fresh > 0;
+    const bool err = seq.len > p->cap && seq.fresh > 0;
     const uint32_t w = err ? (F32 ? 0x7fc00000u : 0x7fff7fffu) : 0u;
-    const int nc = D * ES / 16;
-    for (int u = tid; u < p.H * p.S * nc; u += NT) {
-      const int r = u / nc, h = r / p.S;
-      *(u32x4*)((char*)p.o + (bb * p.o_b + h * p.o_h + (r - h * p.S) * p.o_s) * ES + 16 * (u - r * nc)) = (u32x4){w, w, w, w};
+    const int nc = p->row_b / 16, n = p->U / p->blocks * p->rows * nc;
+    for (int u = tid; u < n; u += NT) {
+      const int r = u / nc, h = quot(r, p->by_s.m, p->by_s.s);
+      *(u32x4*)((char*)p->o + (bb * p->o_b + h * p->o_h + (r - h * p->S) * p->o_s) * ES + 16 * (u - r * nc)) = (u32x4){w, w, w, w};
     }
   }
 }
@@ -683,28 +721,34 @@ int workgroups(int dtype, int B, int H, int Hkv, int S, int D, int page_size, in
   const int64_t units = (int64_t)B * Hkv * ((H / Hkv * S + kRows - 1) / kRows);
   const int64_t cols = n_selected > 0 ? n_selected : width;
   const int64_t tiles = units * cols * ((page_size + kTile - 1) / kTile);
-  const int64_t most = tiles / kMinTiles > units ? tiles / kMinTiles : units;
+  const int64_t most = (tiles + kSetup * units) / kMinTiles > units ? (tiles + kSetup * units) / kMinTiles : units;
   return most < n ? (int)most : n;
 }
 
+Div div_by(int d) {
+  int s = 0;
+  while ((1ll << s) < d) ++s;
+  return {(uint32_t)((1ull << (31 + s)) / (uint32_t)d + 1), s};
+}
+
 template <typename T, int DK>
-hipError_t launch_dk(const PagedAttnParams& p, const Plan& a, int wgs, hipStream_t s) {
+hipError_t launch_dk(const AttnArgs& a, int wgs, hipStream_t s) {
   const dim3 grid(wgs), block(pg_waves(DK * sizeof(T)) * 64);
-  if (p.n_selected > 0) hipLaunchKernelGGL((paged_attn<T, DK, true>), grid, block, 0, s, p, a);
-  else hipLaunchKernelGGL((paged_attn<T, DK, false>), grid, block, 0, s, p, a);
+  if (a.nsel > 0) hipLaunchKernelGGL((paged_attn<T, DK, true>), grid, block, 0, s, a);
+  else hipLaunchKernelGGL((paged_attn<T, DK, false>), grid, block, 0, s, a);
   return hipGetLastError();
 }
 
 template <typename T>
-hipError_t launch16(const PagedAttnParams& p, const Plan& a, int wgs, hipStream_t s) {
-  switch (bucket(0, p.D)) {
-    case 64: return launch_dk<T, 64>(p, a, wgs, s);
-    case 96: return launch_dk<T, 96>(p, a, wgs, s);
-    case 128: return launch_dk<T, 128>(p, a, wgs, s);
-    case 160: return launch_dk<T, 160>(p, a, wgs, s);
-    case 192: return launch_dk<T, 192>(p, a, wgs, s);
+hipError_t launch16(const AttnArgs& a, int wgs, hipStream_t s) {
+  switch (bucket(0, a.D)) {
+    case 64: return launch_dk<T, 64>(a, wgs, s);
+    case 96: return launch_dk<T, 96>(a, wgs, s);
+    case 128: return launch_dk<T, 128>(a, wgs, s);
+    case 160: return launch_dk<T, 160>(a, wgs, s);
+    case 192: return launch_dk<T, 192>(a, wgs, s);
   }
-  return launch_dk<T, 256>(p, a, wgs, s);
+  return launch_dk<T, 256>(a, wgs, s);
 }
 
 }  // namespace
@@ -714,7 +758,7 @@ size_t paged_attn_workspace(int dtype, int B, int H, int Hkv, int S, int D, int 
   // tiles are counted in 32 bits: a table for more is read in whole units
   const int64_t cols = n_selected > 0 ? n_selected : width;
   const int64_t units = (int64_t)B * Hkv * ((H / Hkv * S + kRows - 1) / kRows);
-  if (n <= 1 || units * cols * ((page_size + kTile - 1) / kTile) > INT32_MAX - kMaxWgs) return 0;
+  if (n <= 1 || units * (cols * ((page_size + kTile - 1) / kTile) + kSetup) > INT32_MAX / 2) return 0;
   return kExchangeCounterBytes + (size_t)n * 2 * kRows * (bucket(dtype, D) / 4 + 1) * sizeof(f32x4);
 }
 
@@ -723,20 +767,35 @@ hipError_t launch_paged_attn(const PagedAttnParams& p, int dtype, hipStream_t s)
   const size_t need = paged_attn_workspace(dtype, p.B, p.H, p.Hkv, p.S, p.D, ps, p.map.width, p.n_selected);
   int wgs = workgroups(dtype, p.B, p.H, p.Hkv, p.S, p.D, ps, p.map.width, p.n_selected);
   const int G = p.H / p.Hkv, blocks = (G * p.S + kRows - 1) / kRows, tpp = (ps + kTile - 1) / kTile;
-  Plan a = {nullptr, nullptr, 0, G, blocks, p.Hkv * blocks, tpp};
+  const int es = dtype == 2 ? 4 : 2;
+  AttnArgs a;
+  memset(&a, 0, sizeof a);
+  a.lens = p.map.lens; a.news = p.map.new_lens; a.table = p.map.table; a.selected = p.selected;
+  a.t_str = p.map.stride;
+  a.B = p.B; a.S = p.S; a.U = p.Hkv * blocks; a.cap = p.map.width * ps;
+  a.nsel = p.n_selected; a.width = p.map.width; a.ps = ps; a.tpp = tpp;
+  a.by_ps = div_by(ps); a.by_tpp = div_by(tpp); a.by_blocks = div_by(blocks); a.by_s = div_by(p.S);
+  a.exact = ps % kTile == 0;
+  a.G = G; a.blocks = blocks; a.rows = G * p.S; a.num_pages = p.map.num_pages;
+  a.k = (const char*)p.k; a.v = (const char*)p.v;
+  a.kp_p = p.kp_p * es; a.kp_h = p.kp_h * es; a.vp_p = p.vp_p * es; a.vp_h = p.vp_h * es;
+  a.ks_b = (int)p.kp_s * es; a.vs_b = (int)p.vp_s * es; a.row_b = p.D * es; a.D = p.D;
+  a.q = p.q; a.q_b = p.q_b; a.q_h = p.q_h; a.q_s = p.q_s;
+  a.o = p.o; a.o_b = p.o_b; a.o_h = p.o_h; a.o_s = p.o_s;
+  a.c = p.c; a.q_sign = p.q_sign;
   if (need > 0 && p.workspace && p.workspace_bytes >= need) {
     a.cnt = (int*)p.workspace;
     a.ws = (f32x4*)((char*)p.workspace + kExchangeCounterBytes);
     a.split = 1;
   }
-  if (dtype == 0) return launch16<_Float16>(p, a, wgs, s);
-  if (dtype == 1) return launch16<__bf16>(p, a, wgs, s);
+  if (dtype == 0) return launch16<_Float16>(a, wgs, s);
+  if (dtype == 1) return launch16<__bf16>(a, wgs, s);
   switch (bucket(2, p.D)) {
-    case 64: return launch_dk<float, 64>(p, a, wgs, s);
-    case 128: return launch_dk<float, 128>(p, a, wgs, s);
-    case 192: return launch_dk<float, 192>(p, a, wgs, s);
+    case 64: return launch_dk<float, 64>(a, wgs, s);
+    case 128: return launch_dk<float, 128>(a, wgs, s);
+    case 192: return launch_dk<float, 192>(a, wgs, s);
   }
-  return launch_dk<float, 256>(p, a, wgs, s);
+  return launch_dk<float, 256>(a, wgs, s);
 }
 
 }  // namespace cmpext3
