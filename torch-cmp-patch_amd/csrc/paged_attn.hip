@@ -78,17 +78,26 @@ template <> struct Mma<__bf16> {
 constexpr int kRows = 16;        // query rows of a unit at most
 constexpr int kTile = 16;        // slots of a tile
 constexpr int kMaxWgs = 1024;    // workgroups of a launch at most (counters: one each)
+constexpr int kPerCu = 2;        // workgroups per CU at most
 constexpr int kMinTiles = 16;    // tiles of a workgroup's share at least
 constexpr int kSetup = 6;        // what a unit costs beside its tiles, in tiles
 constexpr int kWhole = 32;       // tiles of a unit that is never split
-constexpr int kMergeLoads = 8;   // loads of one merging thread in flight together
+constexpr int kLongShare = 48;   // tiles of a share from which one workgroup a CU is enough
+constexpr int kMergeLoads = 8;   // parts of one merging thread in flight together
 
-// Waves per workgroup and stages per wave: as many stages as 128 KB of LDS
-// hold, four at most.
+// Waves per workgroup and stages per wave: as many stages as 64 KB of LDS hold,
+// four at most, so that two workgroups fit a CU.  More in flight is no faster
+// (bf16 [16,16/8,4096,128]: 54.3 us with 128 KB a CU, 52.0 with 64).
 constexpr int pg_waves(int rb) { return rb > 512 ? 2 : 4; }  // rb: bytes of a row in LDS
 constexpr int pg_stages(int rb) {
-  const int n = 128 * 1024 / (pg_waves(rb) * 2 * kTile * rb);
-  return n < 4 ? n : 4;
+  const int n = 64 * 1024 / (pg_waves(rb) * 2 * kTile * rb);
+  return n < 1 ? 1 : n < 4 ? n : 4;
+}
+// LDS of a workgroup: the rings, later the waves' states in the same place
+constexpr int pg_lds(int dk, int es) {
+  const int nw = pg_waves(dk * es), ring = nw * pg_stages(dk * es) * 2 * kTile * dk * es;
+  const int states = nw * kRows * (dk + 6) * 4;
+  return ring > states ? ring : states;
 }
 
 // Physical 16-byte chunk of logical chunk c in LDS row r (nc chunks a row): XOR
@@ -122,7 +131,7 @@ struct AttnArgs {
   int B, S, U, cap;        // U: units of a sequence; cap: keys a table row holds
   int nsel, width, ps, tpp;  // tpp: tiles per page
   Div by_ps, by_tpp, by_blocks, by_s;
-  int split, exact;        // split 0: whole units, dealt out in turn; exact: pages are whole tiles
+  int split, exact, full;  // split 0: whole units, dealt out in turn; exact: pages are whole tiles; full: workgroups the CUs hold
   int G, blocks, rows, num_pages;  // query heads per K/V head, row blocks and rows of a K/V head
   const char *k, *v;
   int64_t kp_p, kp_h, vp_p, vp_h;  // bytes
@@ -151,10 +160,10 @@ struct Seq {
   int tiles;       // 0: nothing of it is read (no tokens, no new ones, or longer than its table row)
 };
 template <bool SEL>
-__device__ __forceinline__ Seq seq_of(ArgsPtr p, int b) {
+__device__ __forceinline__ Seq seq_from(ArgsPtr p, int len, int fresh) {
   Seq s;
-  s.len = min(max(p->lens[b], 0), p->cap + 1);
-  s.fresh = min(p->news ? min(max(p->news[b], 0), p->S) : p->S, s.len);
+  s.len = min(max(len, 0), p->cap + 1);
+  s.fresh = min(min(max(fresh, 0), p->S), s.len);
   if (s.fresh == 0 || s.len > p->cap) s.tiles = 0;
   else if (SEL) s.tiles = p->nsel * p->tpp;
   else if (p->exact) s.tiles = (s.len + kTile - 1) / kTile;
@@ -163,6 +172,11 @@ __device__ __forceinline__ Seq seq_of(ArgsPtr p, int b) {
     s.tiles = full * p->tpp + (s.len - full * p->ps + kTile - 1) / kTile;
   }
   return s;
+}
+
+template <bool SEL>
+__device__ __forceinline__ Seq seq_of(ArgsPtr p, int b) {
+  return seq_from<SEL>(p, p->lens[b], p->news ? p->news[b] : p->S);
 }
 
 // Sum over the lanes up to this one.
@@ -177,6 +191,15 @@ __device__ __forceinline__ int wave_scan(int v) {
 }
 
 __device__ __forceinline__ float xor_f(float x, int m) { return __shfl_xor(x, m); }
+// max / sum over the lanes 16 and 32 apart
+__device__ __forceinline__ float rows_max(float x) {
+  const auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+  return xhalf_max(fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1])));
+}
+__device__ __forceinline__ float rows_sum(float x) {
+  const auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+  return xhalf_sum(__uint_as_float(r[0]) + __uint_as_float(r[1]));
+}
 
 template <typename T, int DK, bool SEL>
 __global__ __launch_bounds__(pg_waves(DK * sizeof(T)) * 64, 1) void paged_attn(AttnArgs) {
@@ -196,8 +219,9 @@ __global__ __launch_bounds__(pg_waves(DK * sizeof(T)) * 64, 1) void paged_attn(A
   constexpr int RING = NW * NS * STAGE;
   static_assert(BLK % 1024 == 0 && NC % 4 == 0 && (!F32 || DK % 64 == 0), "head dim bucket");
   static_assert(NS >= 1 && IPT * (NS - 1) <= 63, "vmcnt range");
-  static_assert(NW * kRows * MOS * 4 + 2 * NW * kRows * 4 + 16 <= RING, "the waves' states fit the ring");
-  __shared__ __attribute__((aligned(16))) unsigned char lds[RING];
+  constexpr int LDS = pg_lds(DK, ES);   // the ring, then the waves' states
+  static_assert(LDS >= RING && LDS >= NW * kRows * (MOS + 2) * 4, "the waves' states fit");
+  __shared__ __attribute__((aligned(16))) unsigned char lds[LDS];
   __shared__ int s_flag;
 
   const int tid = thread_x(), lane = tid & 63;
@@ -206,59 +230,13 @@ __global__ __launch_bounds__(pg_waves(DK * sizeof(T)) * 64, 1) void paged_attn(A
   const int c = lane & 15, g = lane >> 4;
   const ArgsPtr args = (ArgsPtr)__builtin_amdgcn_kernarg_segment_ptr();
 
-  // ---- this workgroup's share [lo, hi) of all units, counted in tiles (plus
-  // kSetup for each unit's own cost).  Every wave sums over the batch by itself
-  // (a lane takes `per` sequences in a row), so nothing waits.
-  int b = 0, base = 0;  // the sequence at hand, what lies before it
-  int x = 0, hi = 0, share = 1;
-  bool idle = true;     // a sequence has no tiles
-  Seq held = {0, 0, 0};  // B <= 64: lane b's is sequence b
-  auto weight_of = [](int tiles) { return tiles > 0 ? tiles + kSetup : 0; };
-  // sequence i of the batch, the same for every lane
-  auto seq_at = [&](int i) {
-    Seq s = held;
-    const ArgsPtr p = anew(args);
-    if (p->B > 64) {
-      s = seq_of<SEL>(p, i);
-      i = 0;
-    }
-    s.len = __builtin_amdgcn_readlane(s.len, i);
-    s.fresh = __builtin_amdgcn_readlane(s.fresh, i);
-    s.tiles = __builtin_amdgcn_readlane(s.tiles, i);
-    return s;
-  };
+  // the lane's own lengths are on their way while the offsets below are made
+  int my_len = 0, my_new = 0;
   {
     const ArgsPtr p = anew(args);
-    const int B = p->B, U = p->U, per = (B + 63) >> 6;
-    int sum = 0, busy = 0;
-    for (int k = 0, i = lane * per; k < per; ++k, ++i) {
-      if (i < B) {
-        held = seq_of<SEL>(p, i);
-        sum += weight_of(held.tiles);
-        busy += held.tiles > 0;
-      }
-    }
-    if (p->split) {
-      const int inc = wave_scan(sum);
-      const int total = __builtin_amdgcn_readlane(inc, 63) * U;
-      const int all = __builtin_amdgcn_readlane(wave_scan(busy), 63);
-      idle = all < B;
-      // as many shares as workgroups, but of kMinTiles at least, or a unit each
-      const int n = min(nwg, max(total / kMinTiles, all * U));
-      if (wg < n) {
-        share = (int)(((uint32_t)total + (uint32_t)n - 1u) / (uint32_t)n);
-        x = wg * share;
-        hi = min(x + share, total);
-        const uint64_t in = __builtin_amdgcn_ballot_w64((inc - sum) * U <= x && x < inc * U);
-        if (x < hi) {
-          const int at = (int)__builtin_ctzll(in);
-          base = __builtin_amdgcn_readlane(inc - sum, at) * U;
-          b = at * per;
-        }
-      }
-    } else {
-      x = wg;
-      hi = B * U;
+    if (lane < p->B) {
+      my_len = p->lens[lane];
+      my_new = p->news ? p->news[lane] : p->S;
     }
   }
 
@@ -289,6 +267,76 @@ __global__ __launch_bounds__(pg_waves(DK * sizeof(T)) * 64, 1) void paged_attn(A
   float* const mo = (float*)lds;
   float* const mm = mo + NW * kRows * MOS;
   float* const ml = mm + NW * kRows;
+  // ---- this workgroup's share [lo, hi) of all units, counted in tiles (plus
+  // kSetup for each unit's own cost).  Every wave sums over the batch by itself
+  // (a lane takes `per` sequences in a row), so nothing waits.
+  int b = 0, base = 0;  // the sequence at hand, what lies before it
+  int x = 0, hi = 0, share = 1;
+  bool idle = true;     // a sequence has no tiles
+  int depth = NS;       // stages in use
+  Seq held = {0, 0, 0};  // B <= 64: lane b's is sequence b
+  auto weight_of = [](int tiles) { return tiles > 0 ? tiles + kSetup : 0; };
+  // sequence i of the batch, the same for every lane
+  auto seq_at = [&](int i) {
+    Seq s = held;
+    const ArgsPtr p = anew(args);
+    if (p->B > 64) {
+      s = seq_of<SEL>(p, i);
+      i = 0;
+    }
+    s.len = __builtin_amdgcn_readlane(s.len, i);
+    s.fresh = __builtin_amdgcn_readlane(s.fresh, i);
+    s.tiles = __builtin_amdgcn_readlane(s.tiles, i);
+    return s;
+  };
+  {
+    const ArgsPtr p = anew(args);
+    const int B = p->B, U = p->U, per = (B + 63) >> 6;
+    int sum = 0, busy = 0;
+    if (per == 1) {
+      held = seq_from<SEL>(p, my_len, my_new);
+      sum = weight_of(held.tiles);
+      busy = held.tiles > 0;
+    } else {
+      for (int k = 0, i = lane * per; k < per && i < B; ++k, ++i) {
+        const int t = seq_of<SEL>(p, i).tiles;
+        sum += weight_of(t);
+        busy += t > 0;
+      }
+    }
+    if (p->split) {
+      const int inc = wave_scan(sum);
+      const int total = __builtin_amdgcn_readlane(inc, 63) * U;
+      const int all = __builtin_amdgcn_readlane(wave_scan(busy), 63);
+      idle = all < B;
+      // as many shares as workgroups, but of kMinTiles at least, or a unit each
+      int n = min(nwg, max(total / kMinTiles, all * U));
+      // Two workgroups a CU, one setting up or joining while the other streams:
+      // each with half of its stages, as what waits in the memory's queues
+      // delays whatever a set-up needs (ragged fp16 batch 53.4 us with all, 48.7
+      // with half).  Where units are long and few, nothing but the sweep counts:
+      // one workgroup with all stages (bf16 [16,16/8,4096,128] 54.3 -> 52.0 us).
+      if (n == p->full) {
+        if (all * U < n / 2 && total / (n / 2) >= kLongShare) n /= 2;
+        else depth = (NS + 1) / 2;
+      }
+      if (wg < n) {
+        share = (int)(((uint32_t)total + (uint32_t)n - 1u) / (uint32_t)n);
+        x = wg * share;
+        hi = min(x + share, total);
+        const uint64_t in = __builtin_amdgcn_ballot_w64((inc - sum) * U <= x && x < inc * U);
+        if (x < hi) {
+          const int at = (int)__builtin_ctzll(in);
+          base = __builtin_amdgcn_readlane(inc - sum, at) * U;
+          b = at * per;
+        }
+      }
+    } else {
+      x = wg;
+      hi = B * U;
+    }
+  }
+
   auto weight = [](float m, float mx) { return m == -INFINITY ? 0.f : fast_exp2(m - mx); };
 
   while (x < hi) {
@@ -342,6 +390,55 @@ __global__ __launch_bounds__(pg_waves(DK * sizeof(T)) * 64, 1) void paged_attn(A
       col = row0 + r - h * p->S;
       return head0 + h;
     };
+    // ---- what this wave's tiles [64 k, 64 k + 64) read, lane l's that of tile
+    // 64 k + l: the page's address at the tile's first slot and the bytes from
+    // there that hold keys (K and V), the position of the first key and the
+    // tile's slots
+    uint32_t ka[2], va[2];
+    int kn = 0, vn = 0, pos0 = 0, slots0 = 0;
+    bool bad = false;
+    int page = -1, first = 0;  // between the two steps
+    auto look_up = [&](int k) {
+      const ArgsPtr p = anew(args);
+      const int j = 64 * k + lane, t = ta + wave + NW * j;
+      page = -1;
+      pos0 = first = 0;
+      if (j < mine) {
+        const int e = quot(t, p->by_tpp.m, p->by_tpp.s);
+        first = (t - e * p->tpp) * kTile;
+        const int col = SEL ? p->selected[((int64_t)b * (p->U / p->blocks) + hk) * p->nsel + e] : e;
+        pos0 = -1;
+        if (col >= 0) {
+          pos0 = (int64_t)col * p->ps < len ? col * p->ps + first : 0;
+          if (!SEL || (int64_t)col * p->ps < len) page = p->table[b * p->t_str + col];
+        }
+      }
+    };
+    auto take = [&](int k) {
+      const ArgsPtr p = anew(args);
+      kn = vn = slots0 = 0;
+      const bool wanted = 64 * k + lane < mine && pos0 >= 0;
+      if (page < 0 || page >= p->num_pages) {
+        bad |= wanted;
+        page = -1;
+      } else if (wanted) {
+        slots0 = min(min(kTile, p->ps - first), max(len - pos0, 0));
+      }
+      pos0 = max(pos0, 0);
+      const int ks_b = p->ks_b, vs_b = p->vs_b;
+      if (slots0 > 0) {
+        kn = (slots0 - 1) * ks_b + p->row_b;
+        vn = (slots0 - 1) * vs_b + p->row_b;
+      }
+      const uint64_t kb = (uint64_t)(p->k + max(page, 0) * p->kp_p + hk * p->kp_h + (int64_t)first * ks_b);
+      const uint64_t vb = (uint64_t)(p->v + max(page, 0) * p->vp_p + hk * p->vp_h + (int64_t)first * vs_b);
+      ka[0] = (uint32_t)kb;
+      ka[1] = (uint32_t)(kb >> 32) & 0xffffu;
+      va[0] = (uint32_t)vb;
+      va[1] = (uint32_t)(vb >> 32) & 0xffffu;
+    };
+    look_up(0);
+
     // row c sees the keys before `limit`; every row those before `sure`
     int limit = 0;
     const int sure = S == 1 ? len : 0;
@@ -362,46 +459,6 @@ __global__ __launch_bounds__(pg_waves(DK * sizeof(T)) * 64, 1) void paged_attn(A
       }
     }
 
-    // ---- what this wave's tiles [64 k, 64 k + 64) read, lane l's that of tile
-    // 64 k + l: the page's address at the tile's first slot and the bytes from
-    // there that hold keys (K and V), the position of the first key and the
-    // tile's slots
-    uint32_t ka[2], va[2];
-    int kn = 0, vn = 0, pos0 = 0, slots0 = 0;
-    bool bad = false;
-    auto fetch = [&](int k) {
-      const ArgsPtr p = anew(args);
-      const int j = 64 * k + lane, t = ta + wave + NW * j;
-      int page = -1;
-      kn = vn = pos0 = slots0 = 0;
-      int slot = 0;
-      if (j < mine) {
-        const int e = quot(t, p->by_tpp.m, p->by_tpp.s);
-        slot = (t - e * p->tpp) * kTile;
-        const int col = SEL ? p->selected[((int64_t)b * (p->U / p->blocks) + hk) * p->nsel + e] : e;
-        if (col >= 0) {
-          if (!SEL || (int64_t)col * p->ps < len) page = p->table[b * p->t_str + col];
-          if (page < 0 || page >= p->num_pages) {
-            page = -1;
-            bad = true;
-          } else {
-            pos0 = col * p->ps + slot;
-            slots0 = min(min(kTile, p->ps - slot), max(len - pos0, 0));
-          }
-        }
-      }
-      const int ks_b = p->ks_b, vs_b = p->vs_b;
-      if (slots0 > 0) {
-        kn = (slots0 - 1) * ks_b + p->row_b;
-        vn = (slots0 - 1) * vs_b + p->row_b;
-      }
-      const uint64_t kb = (uint64_t)(p->k + max(page, 0) * p->kp_p + hk * p->kp_h + (int64_t)slot * ks_b);
-      const uint64_t vb = (uint64_t)(p->v + max(page, 0) * p->vp_p + hk * p->vp_h + (int64_t)slot * vs_b);
-      ka[0] = (uint32_t)kb;
-      ka[1] = (uint32_t)(kb >> 32) & 0xffffu;
-      va[0] = (uint32_t)vb;
-      va[1] = (uint32_t)(vb >> 32) & 0xffffu;
-    };
     auto at_lane = [](uint32_t v, int l) { return (uint32_t)__builtin_amdgcn_readlane((int)v, l); };
     // this wave's tile j into stage j % NS
     auto issue = [&](int j) {
@@ -421,14 +478,14 @@ __global__ __launch_bounds__(pg_waves(DK * sizeof(T)) * 64, 1) void paged_attn(A
     float m_run = -INFINITY, l_run = 0.f;
     const float cmul = anew(args)->c;
 
-    fetch(0);
+    take(0);
     // (position, slots) of the tiles in flight: the lanes move on to the next 64
     // tiles when the first of those is issued, up to NS tiles ahead
     int pos_q[NS], slots_q[NS];
 #pragma unroll
     for (int j = 0; j < NS; ++j) {
       pos_q[j] = slots_q[j] = 0;
-      if (j < mine) {
+      if (j < mine && j < depth) {
         pos_q[j] = __builtin_amdgcn_readlane(pos0, j);
         slots_q[j] = __builtin_amdgcn_readlane(slots0, j);
         issue(j);
@@ -436,10 +493,10 @@ __global__ __launch_bounds__(pg_waves(DK * sizeof(T)) * 64, 1) void paged_attn(A
     }
 
     for (int j = 0; j < mine; ++j) {
-      const int behind = min(NS - 1, mine - 1 - j);
-      if (behind >= 3) wait_vmcnt<3 * IPT <= 63 ? 3 * IPT : 63>();
-      else if (behind == 2) wait_vmcnt<2 * IPT <= 63 ? 2 * IPT : 63>();
-      else if (behind == 1) wait_vmcnt<IPT <= 63 ? IPT : 63>();
+      const int behind = min(depth - 1, mine - 1 - j);
+      if (NS > 3 && behind == 3) wait_vmcnt<(NS > 3 ? 3 * IPT : 0)>();
+      else if (NS > 2 && behind == 2) wait_vmcnt<(NS > 2 ? 2 * IPT : 0)>();
+      else if (NS > 1 && behind == 1) wait_vmcnt<(NS > 1 ? IPT : 0)>();
       else wait_vmcnt<0>();
       const unsigned char* st = lds + (wave * NS + j % NS) * STAGE;
       const int pos = pos_q[0], slots = slots_q[0];
@@ -469,9 +526,7 @@ __global__ __launch_bounds__(pg_waves(DK * sizeof(T)) * 64, 1) void paged_attn(A
         for (int e = 0; e < 4; ++e)
           if (4 * g + e >= slots || pos + 4 * g + e >= limit) xs[e] = -INFINITY;
       }
-      float mt = fmaxf(fmaxf(xs[0], xs[1]), fmaxf(xs[2], xs[3]));
-      mt = fmaxf(mt, xor_f(mt, 16));
-      mt = fmaxf(mt, xor_f(mt, 32));
+      const float mt = rows_max(fmaxf(fmaxf(xs[0], xs[1]), fmaxf(xs[2], xs[3])));
       if (__builtin_amdgcn_ballot_w64(mt > m_run)) {  // some row's maximum rises
         const float m_new = fmaxf(m_run, mt);
         const float alpha = weight(m_run, m_new);
@@ -518,19 +573,27 @@ __global__ __launch_bounds__(pg_waves(DK * sizeof(T)) * 64, 1) void paged_attn(A
           oacc[db] = Mma<T>::pv(__builtin_bit_cast(u32x2, v), pl, oacc[db]);
         }
       }
-      if (j + NS < mine) {
-        if (((j + NS) & 63) == 0) fetch((j + NS) >> 6);
-        pos_q[NS - 1] = __builtin_amdgcn_readlane(pos0, (j + NS) & 63);
-        slots_q[NS - 1] = __builtin_amdgcn_readlane(slots0, (j + NS) & 63);
+      const int ahead = j + depth;
+      if (ahead < mine) {
+        if ((ahead & 63) == 0) {
+          look_up(ahead >> 6);
+          take(ahead >> 6);
+        }
+#pragma unroll
+        for (int q = 0; q < NS; ++q) {
+          if (q == depth - 1) {
+            pos_q[q] = __builtin_amdgcn_readlane(pos0, ahead & 63);
+            slots_q[q] = __builtin_amdgcn_readlane(slots0, ahead & 63);
+          }
+        }
         // this stage's LDS reads have returned before its next tile's loads go out
         asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-        issue(j + NS);
+        issue(ahead);
       }
     }
 
     // ---- the waves' states meet in LDS: [wave][row][DK] O, then m, l
-    float lrow = l_run + xor_f(l_run, 16);
-    lrow += xor_f(lrow, 32);
+    float lrow = rows_sum(l_run);
     if (__builtin_amdgcn_ballot_w64(bad)) lrow = __builtin_nanf("");  // a page that is none: the unit's rows are NaN
     wait_vmcnt<0>();
     lds_barrier();  // every wave is done with its ring
@@ -623,8 +686,32 @@ __global__ __launch_bounds__(pg_waves(DK * sizeof(T)) * 64, 1) void paged_attn(A
       // order: the same result whichever workgroup joins.
       auto ld = [&](int off) { return __builtin_bit_cast(f32x4, __builtin_amdgcn_raw_buffer_load_b128(wsr, off, 0, 16)); };
       const int n = parts;
+      if (n <= kMergeLoads) {
+        // few parts: every thread loads all of its vectors and their (m, l) at once
+        for (int u = tid; u < nu; u += NT) {
+          const int r = u / DQ, k = u - r * DQ;
+          f32x4 e[kMergeLoads], v[kMergeLoads];
+#pragma unroll
+          for (int q = 0; q < kMergeLoads; ++q) {
+            const int at = min(q, n - 1);
+            e[q] = ld(slot(at, r, DQ));
+            v[q] = ld(slot(at, r, k));
+          }
+          float mx = -INFINITY, L = 0.f;
+#pragma unroll
+          for (int q = 0; q < kMergeLoads; ++q) mx = fmaxf(mx, e[q][0]);
+          f32x4 o = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+          for (int q = 0; q < kMergeLoads; ++q) {
+            const float f = q < n ? weight(e[q][0], mx) : 0.f;
+            if (q < n) L = __builtin_fmaf(e[q][1], f, L);
+            if (q < n) o += v[q] * f;
+          }
+          store_out(r, k, o, inverse(L));
+        }
+      } else {
       // rows at a time, so that their weights fit the ring's LDS whatever the parts
-      const int rstep = min(R, max(1, (RING - NT * 16 - 64) / (8 * n)));
+      const int rstep = min(R, max(1, (LDS - NT * 16 - 64) / (8 * n)));
       for (int r0 = 0; r0 < R; r0 += rstep) {
         const int rn = min(rstep, R - r0);
         float* const wq = (float*)lds;  // [row][part]
@@ -687,6 +774,7 @@ __global__ __launch_bounds__(pg_waves(DK * sizeof(T)) * 64, 1) void paged_attn(A
         }
         lds_barrier();  // the weights have been read
       }
+      }
     }
     lds_barrier();  // the LDS is free for the next segment
   }
@@ -711,13 +799,16 @@ int bucket(int dtype, int D) {
   return D <= 64 ? 64 : D <= 160 ? (D + 31) / 32 * 32 : (D + 63) / 64 * 64;
 }
 
+// Workgroups that the CUs hold at once.
+int full_house(int dtype, int D) {
+  const int n = device_cus() * min(kPerCu, 160 * 1024 / (pg_lds(bucket(dtype, D), dtype == 2 ? 4 : 2) + 512));
+  return n < kMaxWgs ? n : kMaxWgs;
+}
+
 // Workgroups of a launch: what the CUs hold at once, or fewer when the table
 // rows do not hold that many shares of kMinTiles tiles.
 int workgroups(int dtype, int B, int H, int Hkv, int S, int D, int page_size, int width, int n_selected) {
-  const int rb = bucket(dtype, D) * (dtype == 2 ? 4 : 2);
-  const int lds = pg_waves(rb) * pg_stages(rb) * 2 * kTile * rb;
-  int n = device_cus() * (160 * 1024 / (lds + 4096));
-  if (n > kMaxWgs) n = kMaxWgs;
+  const int n = full_house(dtype, D);
   const int64_t units = (int64_t)B * Hkv * ((H / Hkv * S + kRows - 1) / kRows);
   const int64_t cols = n_selected > 0 ? n_selected : width;
   const int64_t tiles = units * cols * ((page_size + kTile - 1) / kTile);
@@ -776,6 +867,7 @@ hipError_t launch_paged_attn(const PagedAttnParams& p, int dtype, hipStream_t s)
   a.nsel = p.n_selected; a.width = p.map.width; a.ps = ps; a.tpp = tpp;
   a.by_ps = div_by(ps); a.by_tpp = div_by(tpp); a.by_blocks = div_by(blocks); a.by_s = div_by(p.S);
   a.exact = ps % kTile == 0;
+  a.full = full_house(dtype, p.D);
   a.G = G; a.blocks = blocks; a.rows = G * p.S; a.num_pages = p.map.num_pages;
   a.k = (const char*)p.k; a.v = (const char*)p.v;
   a.kp_p = p.kp_p * es; a.kp_h = p.kp_h * es; a.vp_p = p.vp_p * es; a.vp_h = p.vp_h * es;
