@@ -186,6 +186,7 @@ int cmpext3_paged_select(const void* q, const void* key_bounds, int32_t* selecte
   if (n_selected < 1) return CMPEXT3_E_INVALID;
   if ((int64_t)B * H_kv * n_selected > INT32_MAX / 2 || (int64_t)B * H_kv * (table_width + 64ll) > INT32_MAX / 2)
     return CMPEXT3_E_TOO_LARGE;
+  if (B > 65535 || H_kv > 65535) return CMPEXT3_E_TOO_LARGE;  // grid
   if (B == 0) return CMPEXT3_OK;
   if (!selected) return CMPEXT3_E_INVALID;
   CHECKED(check_tensor(q, q_str, B, H, 1, es));

@@ -59,6 +59,9 @@ size_t paged_attn_workspace(int dtype, int B, int H, int Hkv, int S, int D, int 
 hipError_t launch_paged_select(const SelectParams& p, int dtype, hipStream_t s);
 size_t paged_select_workspace(int B, int Hkv, int width);
 
+__device__ __forceinline__ int block_y() { return (int)__builtin_amdgcn_workgroup_id_y(); }
+__device__ __forceinline__ int block_z() { return (int)__builtin_amdgcn_workgroup_id_z(); }
+
 // Tokens of sequence b (0: none), and how many of the S columns are new.
 __device__ __forceinline__ int seq_len(const PageMap& m, int b) { return max(m.lens[b], 0); }
 // The same for readers: a sequence longer than its table row (an error) as one
