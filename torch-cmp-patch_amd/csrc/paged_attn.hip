@@ -179,17 +179,6 @@ __device__ __forceinline__ Seq seq_of(ArgsPtr p, int b) {
   return seq_from<SEL>(p, p->lens[b], p->news ? p->news[b] : p->S);
 }
 
-// Sum over the lanes up to this one.
-__device__ __forceinline__ int wave_scan(int v) {
-  v += __builtin_amdgcn_update_dpp(0, v, 0x111, 0xf, 0xf, false);  // row_shr 1, 2, 4, 8
-  v += __builtin_amdgcn_update_dpp(0, v, 0x112, 0xf, 0xf, false);
-  v += __builtin_amdgcn_update_dpp(0, v, 0x114, 0xf, 0xf, false);
-  v += __builtin_amdgcn_update_dpp(0, v, 0x118, 0xf, 0xf, false);
-  v += __builtin_amdgcn_update_dpp(0, v, 0x142, 0xa, 0xf, false);  // row_bcast 15, 31
-  v += __builtin_amdgcn_update_dpp(0, v, 0x143, 0xc, 0xf, false);
-  return v;
-}
-
 __device__ __forceinline__ float xor_f(float x, int m) { return __shfl_xor(x, m); }
 // max / sum over the lanes 16 and 32 apart
 __device__ __forceinline__ float rows_max(float x) {

@@ -62,6 +62,17 @@ size_t paged_select_workspace(int B, int Hkv, int width);
 __device__ __forceinline__ int block_y() { return (int)__builtin_amdgcn_workgroup_id_y(); }
 __device__ __forceinline__ int block_z() { return (int)__builtin_amdgcn_workgroup_id_z(); }
 
+// Sum over the lanes up to this one.
+__device__ __forceinline__ int wave_scan(int v) {
+  v += __builtin_amdgcn_update_dpp(0, v, 0x111, 0xf, 0xf, false);  // row_shr 1, 2, 4, 8
+  v += __builtin_amdgcn_update_dpp(0, v, 0x112, 0xf, 0xf, false);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x114, 0xf, 0xf, false);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x118, 0xf, 0xf, false);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x142, 0xa, 0xf, false);  // row_bcast 15, 31
+  v += __builtin_amdgcn_update_dpp(0, v, 0x143, 0xc, 0xf, false);
+  return v;
+}
+
 // Tokens of sequence b (0: none), and how many of the S columns are new.
 __device__ __forceinline__ int seq_len(const PageMap& m, int b) { return max(m.lens[b], 0); }
 // The same for readers: a sequence longer than its table row (an error) as one

@@ -27,6 +27,7 @@ namespace {
 constexpr uint64_t kBest = ~0ull;
 constexpr int kSteps = 4;     // steps of pages of a wave, all in flight together
 constexpr int kBins = 2048;
+constexpr int kShort = 1024;  // pages of a row that one launch scores and chooses
 
 // Order of doubles as order of unsigned integers; NaN above everything.
 __device__ __forceinline__ uint64_t order_of(double x) {
@@ -67,26 +68,20 @@ __device__ __forceinline__ double group_sum(double x) {
   return x;
 }
 
-template <typename T, int LG>
-__global__ __launch_bounds__(256) void paged_scores(SelectParams p, uint64_t* keys) {
-  constexpr int N = 16 / sizeof(T);  // elements of a chunk
-  constexpr int PW = 64 / LG;        // pages of a wave's step
-  const int hk = block_y(), b = block_z(), G = p.H / p.Hkv;
-  const int lane = thread_x() & 63, wave = thread_x() >> 6;
-  const int pages = pages_of(p.map, b);
-  const int c0 = (block_x() * 4 + wave) * kSteps * PW + lane / LG;
-  if (block_x() * 4 * kSteps * PW >= pages) return;
-  const int c = lane & (LG - 1);
-  const bool on = c * N < p.D;
-
-  int page[kSteps];
-#pragma unroll
-  for (int s = 0; s < kSteps; ++s) page[s] = c0 + s * PW < pages ? page_at(p.map, b, c0 + s * PW) : -1;
-
+// Q+ and Q- of a K/V head in the 16-byte chunk c.
+template <typename T>
+struct Weights {
+  static constexpr int N = 16 / sizeof(T);  // elements of a chunk
   double up[N], down[N];
+  int c;
+  bool on;
+  __device__ __forceinline__ void load(const SelectParams& p, int b, int hk, int chunk) {
+    const int G = p.H / p.Hkv;
+    c = chunk;
+    on = c * N < p.D;
 #pragma unroll
-  for (int e = 0; e < N; ++e) up[e] = down[e] = 0;
-  if (on) {
+    for (int e = 0; e < N; ++e) up[e] = down[e] = 0;
+    if (!on) return;
     const T* q = (const T*)p.q + b * p.q_b + hk * G * p.q_h + c * N;
     for (int g = 0; g < G; ++g) {
       const u32x4 w = *(const u32x4*)(q + g * p.q_h);
@@ -98,23 +93,41 @@ __global__ __launch_bounds__(256) void paged_scores(SelectParams p, uint64_t* ke
       }
     }
   }
+};
+
+// The bounds of kSteps steps of 64 / LG pages from this lane's column col0 on, on
+// their way while the weights are made.
+template <typename T, int LG>
+struct Bounds {
+  int page[kSteps];
   u32x4 lo[kSteps], hi[kSteps];
+  __device__ __forceinline__ void load(const SelectParams& p, int b, int hk, int col0, int pages, int c) {
+    constexpr int N = 16 / sizeof(T), PW = 64 / LG;
 #pragma unroll
-  for (int s = 0; s < kSteps; ++s) {
-    lo[s] = hi[s] = (u32x4){0u, 0u, 0u, 0u};
-    if (on && page[s] >= 0) {
-      const T* at = (const T*)p.bounds + page[s] * p.kb_p + hk * p.kb_h + c * N;
-      lo[s] = *(const u32x4*)at;
-      hi[s] = *(const u32x4*)(at + p.kb_e);
+    for (int s = 0; s < kSteps; ++s) page[s] = col0 + s * PW < pages ? page_at(p.map, b, col0 + s * PW) : -1;
+#pragma unroll
+    for (int s = 0; s < kSteps; ++s) {
+      lo[s] = hi[s] = (u32x4){0u, 0u, 0u, 0u};
+      if (c * N < p.D && page[s] >= 0) {
+        const T* at = (const T*)p.bounds + page[s] * p.kb_p + hk * p.kb_h + c * N;
+        lo[s] = *(const u32x4*)at;
+        hi[s] = *(const u32x4*)(at + p.kb_e);
+      }
     }
   }
+};
+
+// put(column, key) of those pages.
+template <typename T, int LG, typename Put>
+__device__ __forceinline__ void score_pages(const Bounds<T, LG>& bd, const Weights<T>& w, int col0, int pages, Put put) {
+  constexpr int N = Weights<T>::N, PW = 64 / LG;
 #pragma unroll
   for (int s = 0; s < kSteps; ++s) {
     double sum = 0;
 #pragma unroll
     for (int e = 0; e < N; ++e) {
-      sum = __builtin_fma(up[e], (double)elem<T>(hi[s], e), sum);
-      sum = __builtin_fma(down[e], (double)elem<T>(lo[s], e), sum);
+      sum = __builtin_fma(w.up[e], (double)elem<T>(bd.hi[s], e), sum);
+      sum = __builtin_fma(w.down[e], (double)elem<T>(bd.lo[s], e), sum);
     }
     sum = group_sum<LG>(sum);
     if (__builtin_amdgcn_ballot_w64(sum != sum)) {
@@ -122,16 +135,31 @@ __global__ __launch_bounds__(256) void paged_scores(SelectParams p, uint64_t* ke
       double t = 0;
 #pragma unroll
       for (int e = 0; e < N; ++e) {
-        if (up[e] != 0) t = __builtin_fma(up[e], (double)elem<T>(hi[s], e), t);
-        if (down[e] != 0) t = __builtin_fma(down[e], (double)elem<T>(lo[s], e), t);
+        if (w.up[e] != 0) t = __builtin_fma(w.up[e], (double)elem<T>(bd.hi[s], e), t);
+        if (w.down[e] != 0) t = __builtin_fma(w.down[e], (double)elem<T>(bd.lo[s], e), t);
       }
       t = group_sum<LG>(t);
       if (sum != sum) sum = t;
     }
-    const int col = c0 + s * PW;
-    if (c == 0 && col < pages)
-      keys[((int64_t)b * p.Hkv + hk) * p.map.width + col] = page[s] >= 0 ? order_of(sum) : kBest;
+    const int col = col0 + s * PW;
+    if (w.c == 0 && col < pages) put(col, bd.page[s] >= 0 ? order_of(sum) : kBest);
   }
+}
+
+template <typename T, int LG>
+__global__ __launch_bounds__(256) void paged_scores(SelectParams p, uint64_t* keys) {
+  constexpr int PW = 64 / LG;        // pages of a wave's step
+  const int hk = block_y(), b = block_z();
+  const int lane = thread_x() & 63, wave = thread_x() >> 6;
+  const int pages = pages_of(p.map, b);
+  if (block_x() * 4 * kSteps * PW >= pages) return;
+  const int col0 = (block_x() * 4 + wave) * kSteps * PW + lane / LG;
+  Bounds<T, LG> e;
+  e.load(p, b, hk, col0, pages, lane & (LG - 1));
+  Weights<T> w;
+  w.load(p, b, hk, lane & (LG - 1));
+  uint64_t* row = keys + ((int64_t)b * p.Hkv + hk) * p.map.width;
+  score_pages<T, LG>(e, w, col0, pages, [&](int c, uint64_t k) { row[c] = k; });
 }
 
 __device__ __forceinline__ uint64_t wave_min(uint64_t x) {
@@ -143,28 +171,26 @@ __device__ __forceinline__ uint64_t wave_min(uint64_t x) {
   return x;
 }
 
-// NW waves, each with a contiguous range of columns in steps of 64; HELD: the
-// steps' keys stay in registers, else each round reads them again.
-template <int NW, int HELD>
-__global__ __launch_bounds__(NW * 64) void paged_best(SelectParams p, const uint64_t* all) {
-  __shared__ uint64_t s_min[NW], s_max[NW];
-  __shared__ int hist[kBins];
-  __shared__ int s_sum[NW], s_pick[3], s_gt[NW], s_eq[NW];
+struct BestShared {
+  int hist[kBins];
+  uint64_t mn[16], mx[16], cand[64], key;
+  int cand_col[64], sum[16], pick[3], cands, col;
+};
+
+// The K best columns of a row of `pages` scores, load(column) each, with NW
+// waves that take a contiguous range of columns each, in steps of 64.  HELD:
+// the steps' keys stay in registers, else every round loads them again.
+template <int NW, int HELD, typename Load>
+__device__ __forceinline__ void best(BestShared& sh, int pages, int K, int32_t* out, Load load) {
   const int tid = thread_x(), lane = tid & 63, wave = tid >> 6;
-  const int hk = block_x(), b = block_y(), K = p.n_selected;
-  const int pages = pages_of(p.map, b);
-  const uint64_t* keys = all + ((int64_t)b * p.Hkv + hk) * p.map.width;
-  int32_t* out = p.selected + ((int64_t)b * p.Hkv + hk) * K;
   for (int j = min(pages, K) + tid; j < K; j += NW * 64) out[j] = -1;
   if (pages <= K) {
     for (int j = tid; j < pages; j += NW * 64) out[j] = j;
     return;
   }
   const int m = pages - 1;  // the last page is in; the K - 1 best of m others
-  if (K == 1) {
-    if (tid == 0) out[0] = m;
-    return;
-  }
+  if (tid == 0) out[K - 1] = m;
+  if (K == 1) return;
   const int steps = (m + NW * 64 - 1) / (NW * 64);
   const int first = wave * steps * 64 + lane;
   uint64_t held[HELD > 0 ? HELD : 1];
@@ -172,9 +198,10 @@ __global__ __launch_bounds__(NW * 64) void paged_best(SelectParams p, const uint
 #pragma unroll
     for (int s = 0; s < HELD; ++s) {
       const int c = first + 64 * s;
-      held[s] = s < steps && c < m ? keys[c] : 0;  // 0: below every key
+      held[s] = s < steps && c < m ? load(c) : 0;  // 0: below every key
     }
   }
+  const uint64_t ref = load(0);
   // f(key, column) for this lane's columns
   auto each = [&](auto f) {
     if constexpr (HELD > 0) {
@@ -182,45 +209,70 @@ __global__ __launch_bounds__(NW * 64) void paged_best(SelectParams p, const uint
       for (int s = 0; s < HELD; ++s)
         if (s < steps) f(held[s], first + 64 * s);
     } else {
-      for (int s = 0; s < steps; ++s) f(first + 64 * s < m ? keys[first + 64 * s] : 0, first + 64 * s);
+      for (int s = 0; s < steps; ++s) f(first + 64 * s < m ? load(first + 64 * s) : 0, first + 64 * s);
     }
   };
 
-  // the keys in question are those in [lo, hi]; `need` of them are taken
-  uint64_t lo = 1, hi = kBest;
-  int need = K - 1;
-  bool ties = false;  // all of them are equal
-  for (;;) {
-    uint64_t mn = kBest, mx = 0;
-    each([&](uint64_t k, int) {
-      if (k >= lo && k <= hi) {
-        mn = k < mn ? k : mn;
-        mx = k > mx ? k : mx;
+  // Taken are the keys above `key`, and those equal to it up to column `col`.
+  // The border lies among the keys in [lo, hi], of which `need` are taken.
+  uint64_t lo = 1, hi = kBest, key;
+  int need = K - 1, col = INT32_MAX;
+  for (int round = 0;; ++round) {
+    for (int j = tid; j < kBins; j += NW * 64) sh.hist[j] = 0;
+    int shift = 44;
+    const int64_t zero = (int64_t)(ref >> 44) - kBins / 2;  // the first round's bin 0
+    if (round > 0) {
+      uint64_t mn = kBest, mx = 0;
+      each([&](uint64_t k, int) {
+        if (k >= lo && k <= hi) {
+          mn = k < mn ? k : mn;
+          mx = k > mx ? k : mx;
+        }
+      });
+      mn = wave_min(mn);
+      mx = ~wave_min(~mx);
+      if (lane == 0) {
+        sh.mn[wave] = mn;
+        sh.mx[wave] = mx;
       }
-    });
-    mn = wave_min(mn);
-    mx = ~wave_min(~mx);
-    if (lane == 0) {
-      s_min[wave] = mn;
-      s_max[wave] = mx;
-    }
-    for (int j = tid; j < kBins; j += NW * 64) hist[j] = 0;
-    __syncthreads();
+      __syncthreads();
 #pragma unroll
-    for (int w = 0; w < NW; ++w) {
-      mn = s_min[w] < mn ? s_min[w] : mn;
-      mx = s_max[w] > mx ? s_max[w] : mx;
+      for (int w = 0; w < NW; ++w) {
+        mn = sh.mn[w] < mn ? sh.mn[w] : mn;
+        mx = sh.mx[w] > mx ? sh.mx[w] : mx;
+      }
+      lo = mn;
+      hi = mx;
+      if (lo == hi) {  // equal keys: the `need` lowest columns
+        int eq = 0;
+        each([&](uint64_t k, int) { eq += __builtin_popcountll(__builtin_amdgcn_ballot_w64(k == lo)); });
+        if (lane == 0) sh.sum[wave] = eq;
+        __syncthreads();
+        int before = 0;
+        for (int w = 0; w < wave; ++w) before += sh.sum[w];
+        if (before < need && before + eq >= need)
+          each([&](uint64_t k, int c) {
+            const uint64_t in = __builtin_amdgcn_ballot_w64(k == lo);
+            if (k == lo && before + __builtin_popcountll(in & (lane ? ~0ull >> (64 - lane) : 0ull)) == need - 1) sh.col = c;
+            before += __builtin_popcountll(in);
+          });
+        __syncthreads();
+        key = lo;
+        col = sh.col;
+        break;
+      }
+      const int bits = 64 - __builtin_clzll(hi - lo);
+      shift = bits > 11 ? bits - 11 : 0;
+    } else {
+      __syncthreads();
     }
-    lo = mn;
-    hi = mx;
-    if (lo == hi) {
-      ties = true;
-      break;
-    }
-    const int bits = 64 - __builtin_clzll(hi - lo);
-    const int shift = bits > 11 ? bits - 11 : 0;
+    // Scores of one sequence and head are of one magnitude: the first round takes
+    // 256 bins an octave around one of them, without a look at their range.
     each([&](uint64_t k, int) {
-      if (k >= lo && k <= hi) atomicAdd(&hist[(int)((k - lo) >> shift)], 1);
+      if (k < lo || k > hi) return;
+      int64_t bin = round > 0 ? (int64_t)((k - lo) >> shift) : (int64_t)(k >> 44) - zero;
+      bin = bin < 0 ? 0 : bin > kBins - 1 ? kBins - 1 : bin;
+      atomicAdd(&sh.hist[(int)bin], 1);
     });
     __syncthreads();
     // from the top: the bin in which the count reaches `need`
@@ -228,88 +280,143 @@ __global__ __launch_bounds__(NW * 64) void paged_best(SelectParams p, const uint
     int mine = 0, h[BT];
 #pragma unroll
     for (int j = 0; j < BT; ++j) {
-      h[j] = hist[kBins - 1 - (tid * BT + j)];
+      h[j] = sh.hist[kBins - 1 - (tid * BT + j)];
       mine += h[j];
     }
-    int inc = mine;
-#pragma unroll
-    for (int d = 1; d < 64; d <<= 1) {
-      const int u = __shfl_up(inc, d);
-      if (lane >= d) inc += u;
-    }
-    if (lane == 63) s_sum[wave] = inc;
+    int inc = wave_scan(mine);
+    if (lane == 63) sh.sum[wave] = inc;
+    if (tid == 0) sh.cands = 0;
     __syncthreads();
     int above = inc - mine;
-    for (int w = 0; w < wave; ++w) above += s_sum[w];
+    for (int w = 0; w < wave; ++w) above += sh.sum[w];
 #pragma unroll
     for (int j = 0; j < BT; ++j) {
       if (above < need && above + h[j] >= need) {
-        s_pick[0] = kBins - 1 - (tid * BT + j);
-        s_pick[1] = above;
-        s_pick[2] = h[j];
+        sh.pick[0] = kBins - 1 - (tid * BT + j);
+        sh.pick[1] = above;
+        sh.pick[2] = h[j];
       }
       above += h[j];
     }
     __syncthreads();
-    const uint64_t bin = (uint64_t)s_pick[0];
-    need -= s_pick[1];
-    const int inside = s_pick[2];
-    const uint64_t top = lo + ((bin + 1) << shift) - 1;
-    lo += bin << shift;
-    hi = top < hi && top >= lo ? top : hi;
+    const int bin = sh.pick[0], inside = sh.pick[2];
+    need -= sh.pick[1];
+    if (round > 0) {
+      const uint64_t top = lo + ((uint64_t)(bin + 1) << shift) - 1;
+      lo += (uint64_t)bin << shift;
+      hi = top < hi && top >= lo ? top : hi;
+    } else {  // the outermost bins hold all that lies beyond them
+      if (bin < kBins - 1) hi = (uint64_t)((zero + bin + 1) << 44) - 1;
+      if (bin > 0) lo = (uint64_t)((zero + bin) << 44);
+    }
+    if (inside == need) {  // all of the bin
+      key = lo - 1;
+      col = -1;
+      break;
+    }
+    if (inside <= 64) {  // few: each is compared with all, by NW lanes together
+      each([&](uint64_t k, int c) {
+        if (k >= lo && k <= hi) {
+          const int i = atomicAdd(&sh.cands, 1);
+          sh.cand[i] = k;
+          sh.cand_col[i] = c;
+        }
+      });
+      __syncthreads();
+      const int i = tid / NW;
+      if (i < inside) {
+        const uint64_t k = sh.cand[i];
+        const int c = sh.cand_col[i];
+        int rank = 0;
+        for (int j = tid % NW; j < inside; j += NW) {
+          const uint64_t o = sh.cand[j];
+          rank += o > k || (o == k && sh.cand_col[j] < c);
+        }
+#pragma unroll
+        for (int d = 1; d < NW; d <<= 1) rank += __shfl_xor(rank, d);
+        if (rank == need - 1) {
+          sh.key = k;
+          sh.col = c;
+        }
+      }
+      __syncthreads();
+      key = sh.key;
+      col = sh.col;
+      break;
+    }
     __syncthreads();
-    if (inside == need) break;  // all of the bin
   }
 
-  // taken: keys above hi, and of those in [lo, hi] all, or the first `need`
-  int gt = 0, eq = 0;
-  each([&](uint64_t k, int) {
-    gt += __builtin_popcountll(__builtin_amdgcn_ballot_w64(k > hi));
-    eq += __builtin_popcountll(__builtin_amdgcn_ballot_w64(k >= lo && k <= hi));
-  });
-  if (lane == 0) {
-    s_gt[wave] = gt;
-    s_eq[wave] = eq;
-  }
+  int before = 0;
+  auto taken = [&](uint64_t k, int c) { return k > key || (k == key && c <= col); };
+  each([&](uint64_t k, int c) { before += __builtin_popcountll(__builtin_amdgcn_ballot_w64(taken(k, c))); });
   __syncthreads();
-  gt = eq = 0;
-  for (int w = 0; w < wave; ++w) {
-    gt += s_gt[w];
-    eq += s_eq[w];
-  }
-  const int most = ties ? need : INT32_MAX;
-  const uint64_t below = lane ? ~0ull >> (64 - lane) : 0ull;
+  if (lane == 0) sh.sum[wave] = before;
+  __syncthreads();
+  before = 0;
+  for (int w = 0; w < wave; ++w) before += sh.sum[w];
   each([&](uint64_t k, int c) {
-    const uint64_t g = __builtin_amdgcn_ballot_w64(k > hi), e = __builtin_amdgcn_ballot_w64(k >= lo && k <= hi);
-    const int eb = eq + __builtin_popcountll(e & below);
-    const bool in_e = k >= lo && k <= hi;
-    if (k > hi || (in_e && eb < most)) out[gt + __builtin_popcountll(g & below) + min(eb, most)] = c;
-    gt += __builtin_popcountll(g);
-    eq += __builtin_popcountll(e);
+    const uint64_t in = __builtin_amdgcn_ballot_w64(taken(k, c));
+    if (taken(k, c)) out[before + __builtin_popcountll(in & (lane ? ~0ull >> (64 - lane) : 0ull))] = c;
+    before += __builtin_popcountll(in);
   });
-  if (tid == 0) out[K - 1] = m;
+}
+
+template <int NW, int HELD>
+__global__ __launch_bounds__(NW * 64) void paged_best(SelectParams p, const uint64_t* all) {
+  __shared__ BestShared sh;
+  const int hk = block_x(), b = block_y();
+  const uint64_t* keys = all + ((int64_t)b * p.Hkv + hk) * p.map.width;
+  best<NW, HELD>(sh, pages_of(p.map, b), p.n_selected, p.selected + ((int64_t)b * p.Hkv + hk) * p.n_selected,
+                 [&](int c) { return keys[c]; });
+}
+
+// Both in one launch, a workgroup a row: rows of up to kShort pages.
+template <typename T, int LG>
+__global__ __launch_bounds__(1024) void paged_short(SelectParams p) {
+  __shared__ BestShared sh;
+  __shared__ uint64_t keys[kShort];
+  constexpr int PW = 64 / LG;
+  const int hk = block_x(), b = block_y();
+  const int lane = thread_x() & 63, wave = thread_x() >> 6;
+  const int pages = pages_of(p.map, b);
+  if (pages > p.n_selected && p.n_selected > 1) {
+    Bounds<T, LG> e;
+    e.load(p, b, hk, wave * kSteps * PW + lane / LG, pages, lane & (LG - 1));
+    Weights<T> w;
+    w.load(p, b, hk, lane & (LG - 1));
+    for (int c0 = wave * kSteps * PW; c0 < pages;) {
+      score_pages<T, LG>(e, w, c0 + lane / LG, pages, [&](int c, uint64_t k) { keys[c] = k; });
+      c0 += 16 * kSteps * PW;
+      if (c0 < pages) e.load(p, b, hk, c0 + lane / LG, pages, lane & (LG - 1));
+    }
+    __syncthreads();
+  }
+  best<16, kShort / 1024>(sh, pages, p.n_selected, p.selected + ((int64_t)b * p.Hkv + hk) * p.n_selected,
+                          [&](int c) { return keys[c]; });
 }
 
 template <typename T, int LG>
-void scores(const SelectParams& p, uint64_t* keys, hipStream_t s) {
+void launch_lg(const SelectParams& p, hipStream_t s) {
+  uint64_t* keys = (uint64_t*)p.workspace;
+  const dim3 rows(p.Hkv, p.B);
+  if (p.map.width <= kShort) {
+    hipLaunchKernelGGL((paged_short<T, LG>), rows, dim3(1024), 0, s, p);
+    return;
+  }
   const int per = 4 * kSteps * (64 / LG);
   hipLaunchKernelGGL((paged_scores<T, LG>), dim3((p.map.width + per - 1) / per, p.Hkv, p.B), dim3(256), 0, s, p, keys);
+  if (p.map.width <= 16 * 64 * 8) hipLaunchKernelGGL((paged_best<16, 8>), rows, dim3(1024), 0, s, p, keys);
+  else hipLaunchKernelGGL((paged_best<16, 0>), rows, dim3(1024), 0, s, p, keys);
 }
 
 template <typename T>
 hipError_t launch(const SelectParams& p, hipStream_t s) {
-  uint64_t* keys = (uint64_t*)p.workspace;
   const int chunks = p.D * (int)sizeof(T) / 16;
-  if (p.map.width > 0) {
-    if (chunks <= 8) scores<T, 8>(p, keys, s);
-    else if (chunks <= 16) scores<T, 16>(p, keys, s);
-    else if (chunks <= 32) scores<T, 32>(p, keys, s);
-    else if constexpr (sizeof(T) == 4) scores<T, 64>(p, keys, s);
-  }
-  const dim3 grid(p.Hkv, p.B);
-  if (p.map.width <= 4 * 64 * 4) hipLaunchKernelGGL((paged_best<4, 4>), grid, dim3(256), 0, s, p, keys);
-  else if (p.map.width <= 16 * 64 * 8) hipLaunchKernelGGL((paged_best<16, 8>), grid, dim3(1024), 0, s, p, keys);
-  else hipLaunchKernelGGL((paged_best<16, 0>), grid, dim3(1024), 0, s, p, keys);
+  if (chunks <= 8) launch_lg<T, 8>(p, s);
+  else if (chunks <= 16) launch_lg<T, 16>(p, s);
+  else if (chunks <= 32) launch_lg<T, 32>(p, s);
+  else if constexpr (sizeof(T) == 4) launch_lg<T, 64>(p, s);
   return hipGetLastError();
 }
 
