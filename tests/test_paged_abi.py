@@ -74,7 +74,7 @@ def test_attention_refuses_before_launch(args, code):
     (dict(cos=A, sin=A, rows=4, rot=0), INV), (dict(cos=A + 2, sin=A, rows=4, rot=64, rs=32), AL),
     (dict(cos=A, sin=A, rows=4, rot=64, rs=-32), INV), (dict(cos=A, sin=A, rows=4, rot=64, rs=32, q=A, qo=A), INV),
     (dict(cos=A, sin=A, rows=4, rot=64, rs=32, q=A, qo=A + 4096, H=3), INV), (dict(pos=A + 1), AL),
-    (dict(B=65536, H=2), BIG), (dict(Hkv=40000, B=1), BIG), (dict(ks=s3(128, 64, -1), S=3), INV),
+    (dict(B=1 << 27), BIG), (dict(Hkv=1 << 28, B=1), BIG), (dict(S=1 << 20, page=1, B=16, kb=A), BIG), (dict(ks=s3(128, 64, -1), S=3), INV),
 ])
 def test_append_refuses_before_launch(args, code):
     assert append(**args) == code

@@ -1,11 +1,21 @@
 // Appending new tokens to a paged key-value cache, with the rotary position
 // embedding applied on the way.
 //
-// Work is cut by runs: the new tokens of one sequence that fall into one page.
-// One wave takes a (sequence, run, head) of K, V or Q, a lane one 16-byte chunk
-// of a token's row and as many tokens at a time as chunks fit the wave.  A run
-// ends with its page, so its keys' channel bounds are the wave's own: they are
-// kept in registers, joined over the wave's token lanes and written once.
+// Bound by HBM for prompts (every row is read once and written once) and by
+// the latency of its loads for single tokens: lengths, then the page number
+// and the rotation's row, while the rows themselves, which depend on neither,
+// are on their way.
+//
+// A lane takes one unit of a row: with pairs (d, d + rot / 2) the two 16-byte
+// chunks that turn together, else one chunk.  Lanes run over a token's units,
+// then over its heads (K, V and Q in a row), then over tokens, so that a
+// workgroup reads what a projection left in one stretch and a rotation's row
+// once for all of a token's heads.
+//
+// With key bounds, keys of more than one token a call are taken by runs instead: the new tokens
+// of one sequence that fall into one page.  A wave takes a (sequence, run,
+// head); the run ends with its page, so the page's bounds are the wave's own:
+// kept in registers, joined over the wave's token lanes, written once.
 #include "paged_common.h"
 
 namespace cmpext3 {
@@ -52,132 +62,310 @@ template <> struct Elem<float> {
   static __device__ u32x4 nan() { return (u32x4){0x7fc00000u, 0x7fc00000u, 0x7fc00000u, 0x7fc00000u}; }
 };
 
-// Chunk c of a row, rotated by the angles in (cs, sn): the partner of element
-// d < rot / 2 is d + rot / 2 (or its neighbour, when pairs lie side by side).
-template <typename T>
-__device__ u32x4 rotated(const T* row, int c, const AppendParams& p, const float* cs, const float* sn) {
-  constexpr int N = Elem<T>::N;
-  const u32x4 w = *(const u32x4*)(row + c * N);
-  const int d0 = c * N, h = p.rot / 2;
-  if (d0 >= p.rot) return w;
-  float x[N], o[N];
-#pragma unroll
-  for (int e = 0; e < N; ++e) x[e] = Elem<T>::get(w, e);
-  if (p.interleaved) {
-#pragma unroll
-    for (int e = 0; e < N; e += 2) {
-      const int j = (d0 + e) / 2;
-      const bool in = d0 + e < p.rot;
-      const float a = in ? cs[j] : 1.f, s = in ? sn[j] : 0.f;
-      o[e] = in ? x[e] * a - x[e + 1] * s : x[e];
-      o[e + 1] = in ? x[e + 1] * a + x[e] * s : x[e + 1];
-    }
-  } else {
-#pragma unroll
-    for (int e = 0; e < N; ++e) {
-      const int d = d0 + e;
-      if (d < h) o[e] = x[e] * cs[d] - (float)row[d + h] * sn[d];
-      else if (d < p.rot) o[e] = x[e] * cs[d - h] + (float)row[d - h] * sn[d - h];
-      else o[e] = x[e];
+// How a row is rotated.
+enum Mode {
+  kCopy,   // not at all
+  kHalf,   // pairs (d, d + rot / 2) in whole chunks
+  kSide,   // pairs (2 d, 2 d + 1) in whole chunks
+  kAny     // anything else: element by element
+};
+
+struct Shape {
+  int units, pairs;  // units of a row; the first `pairs` of them are two chunks, `pairs` apart
+  int heads;         // heads of a token in the first section: V and Q, and K where it takes no runs
+  int runs;          // workgroups of the second section per (sequence, 4 heads): 0 without it
+  int first;         // workgroups of the first section
+  int q_at, v_at;    // where V's and Q's heads begin in a token's
+  Div by_units, by_heads, by_s, by_ps, by_runs, by_groups;
+};
+
+// One unit of a row: its chunks, and those rotated.
+template <typename T, int MODE>
+struct Unit {
+  static constexpr int N = Elem<T>::N;
+  int c0, c1;  // c1 < 0: one chunk
+  u32x4 x0, x1;
+  __device__ __forceinline__ Unit(int u, const Shape& sh) {
+    if constexpr (MODE == kHalf) {
+      c0 = u < sh.pairs ? u : u + sh.pairs;
+      c1 = u < sh.pairs ? u + sh.pairs : -1;
+    } else {
+      c0 = u;
+      c1 = -1;
     }
   }
-  return Elem<T>::put(o);
+  __device__ __forceinline__ void load(const T* row) {
+    x0 = *(const u32x4*)(row + c0 * N);
+    x1 = x0;
+    if constexpr (MODE == kHalf) {
+      if (c1 >= 0) x1 = *(const u32x4*)(row + c1 * N);
+    }
+  }
+  // by the angles of one row of the tables
+  __device__ __forceinline__ void rotate(const T* row, const AppendParams& p, const float* cs, const float* sn) {
+    const int d0 = c0 * N;
+    if constexpr (MODE == kHalf) {
+      if (c1 < 0) return;
+      float a[N], b[N];
+      f32x4 c[N / 4], s[N / 4];
+#pragma unroll
+      for (int k = 0; k < N / 4; ++k) {
+        c[k] = *(const f32x4*)(cs + d0 + 4 * k);
+        s[k] = *(const f32x4*)(sn + d0 + 4 * k);
+      }
+#pragma unroll
+      for (int e = 0; e < N; ++e) {
+        const float x = Elem<T>::get(x0, e), y = Elem<T>::get(x1, e), cc = c[e / 4][e % 4], ss = s[e / 4][e % 4];
+        a[e] = x * cc - y * ss;
+        b[e] = y * cc + x * ss;
+      }
+      x0 = Elem<T>::put(a);
+      x1 = Elem<T>::put(b);
+    } else if constexpr (MODE == kSide) {
+      if (d0 >= p.rot) return;
+      float a[N], c[N / 2], s[N / 2];
+      if constexpr (N == 8) {
+        *(f32x4*)c = *(const f32x4*)(cs + d0 / 2);
+        *(f32x4*)s = *(const f32x4*)(sn + d0 / 2);
+      } else {
+        *(u32x2*)c = *(const u32x2*)(cs + d0 / 2);
+        *(u32x2*)s = *(const u32x2*)(sn + d0 / 2);
+      }
+#pragma unroll
+      for (int e = 0; e < N; e += 2) {
+        const float x = Elem<T>::get(x0, e), y = Elem<T>::get(x0, e + 1);
+        a[e] = x * c[e / 2] - y * s[e / 2];
+        a[e + 1] = y * c[e / 2] + x * s[e / 2];
+      }
+      x0 = Elem<T>::put(a);
+    } else if constexpr (MODE == kAny) {
+      const int h = p.rot / 2;
+      if (d0 >= p.rot) return;
+      float a[N];
+#pragma unroll
+      for (int e = 0; e < N; ++e) {
+        const int d = d0 + e;
+        const int j = p.interleaved ? d / 2 : d < h ? d : d - h;
+        const bool low = p.interleaved ? (d & 1) == 0 : d < h;
+        const float x = Elem<T>::get(x0, e);
+        a[e] = x;
+        if (d < p.rot) {
+          const float y = (float)row[p.interleaved ? (low ? d + 1 : d - 1) : (low ? d + h : d - h)];
+          a[e] = low ? x * cs[j] - y * sn[j] : x * cs[j] + y * sn[j];
+        }
+      }
+      x0 = Elem<T>::put(a);
+    }
+  }
+  __device__ __forceinline__ void store(T* row) const {
+    *(u32x4*)(row + c0 * N) = x0;
+    if constexpr (MODE == kHalf) {
+      if (c1 >= 0) *(u32x4*)(row + c1 * N) = x1;
+    }
+  }
+  __device__ __forceinline__ void fill(const u32x4& w) { x0 = x1 = w; }
+};
+
+// Lowest and highest values of one chunk's channels.
+template <typename T>
+struct Range {
+  static constexpr int N = Elem<T>::N;
+  float lo[N], hi[N];
+  __device__ __forceinline__ Range() {
+#pragma unroll
+    for (int e = 0; e < N; ++e) {
+      lo[e] = INFINITY;
+      hi[e] = -INFINITY;
+    }
+  }
+  __device__ __forceinline__ void take(const u32x4& w) {
+#pragma unroll
+    for (int e = 0; e < N; ++e) {
+      lo[e] = fminf(lo[e], Elem<T>::get(w, e));
+      hi[e] = fmaxf(hi[e], Elem<T>::get(w, e));
+    }
+  }
+  // over the lanes of the same unit, `units` apart, `n` of them, into the first
+  __device__ __forceinline__ void join(int lane, int t, int n, int units) {
+    for (int d = 1; d < n; d <<= 1) {
+      const bool in = t + d < n;
+#pragma unroll
+      for (int e = 0; e < N; ++e) {
+        const float l = __shfl(lo[e], (lane + d * units) & 63), h = __shfl(hi[e], (lane + d * units) & 63);
+        lo[e] = in ? fminf(lo[e], l) : lo[e];
+        hi[e] = in ? fmaxf(hi[e], h) : hi[e];
+      }
+    }
+  }
+  __device__ __forceinline__ void store(T* lows, T* highs, bool anew) {
+    if (!anew) {
+      const u32x4 a = *(const u32x4*)lows, z = *(const u32x4*)highs;
+#pragma unroll
+      for (int e = 0; e < N; ++e) {
+        lo[e] = fminf(lo[e], Elem<T>::get(a, e));
+        hi[e] = fmaxf(hi[e], Elem<T>::get(z, e));
+      }
+    }
+    *(u32x4*)lows = Elem<T>::put(lo);
+    *(u32x4*)highs = Elem<T>::put(hi);
+  }
+};
+
+// Keys of a run with their page's bounds.
+template <typename T, int MODE>
+__device__ __forceinline__ void append_run(const AppendParams& p, const Shape& sh, int wg) {
+  constexpr int N = Elem<T>::N;
+  const int lane = thread_x() & 63, wave = __builtin_amdgcn_readfirstlane(thread_x() >> 6);
+  const int rest = quot(wg, sh.by_runs.m, sh.by_runs.s), run = wg - rest * sh.runs;
+  const int groups = (p.Hkv + 3) / 4;
+  const int b = quot(rest, sh.by_groups.m, sh.by_groups.s), head = (rest - b * groups) * 4 + wave;
+  if (head >= p.Hkv) return;
+  const int len = seq_len(p.map, b), n = seq_new(p.map, b, p.S, len);
+  const int pos0 = len - n, ps = p.map.page_size;
+  const int64_t col = (int64_t)quot(pos0, sh.by_ps.m, sh.by_ps.s) + run;
+  const int64_t start = col * ps - pos0;  // the page's slot 0 as a column
+  if (start >= n) return;
+  const int i0 = start > 0 ? (int)start : 0, i1 = start + ps < n ? (int)(start + ps) : n;
+  const int page = page_at(p.map, b, col);
+  if (page < 0) return;
+  const int TL = 64 / sh.units, t = quot(lane, sh.by_units.m, sh.by_units.s), u = lane - t * sh.units;
+  const T* src = (const T*)p.k + b * p.k_b + head * p.k_h;
+  T* dst = (T*)p.k_pages + page * p.kp_p + head * p.kp_h;
+  const Unit<T, MODE> at(u, sh);
+  Range<T> r0, r1;
+  bool some = false;
+  if (t < TL) {
+#pragma unroll 2
+    for (int i = i0 + t; i < i1; i += TL) {
+      const T* row = src + i * p.k_s;
+      Unit<T, MODE> w = at;
+      w.load(row);
+      bool ok = true;
+      if constexpr (MODE != kCopy) {
+        const int a = p.positions ? p.positions[(int64_t)b * p.S + i] : pos0 + i;
+        ok = a >= 0 && a < p.rows;
+        if (ok) w.rotate(row, p, p.cos + a * p.rot_s, p.sin + a * p.rot_s);
+      }
+      if (ok) {
+        w.store(dst + (i - start) * p.kp_s);
+        r0.take(w.x0);
+        if constexpr (MODE == kHalf) r1.take(w.x1);
+        some = true;
+      }
+    }
+  }
+  if (!__builtin_amdgcn_ballot_w64(some)) return;
+  r0.join(lane, t, TL, sh.units);
+  if constexpr (MODE == kHalf) r1.join(lane, t, TL, sh.units);
+  if (t != 0) return;
+  const bool anew = start >= 0;  // the page begins with a new token
+  T* edge = (T*)p.bounds + page * p.kb_p + head * p.kb_h;
+  r0.store(edge + at.c0 * N, edge + p.kb_e + at.c0 * N, anew);
+  if constexpr (MODE == kHalf) {
+    if (at.c1 >= 0) r1.store(edge + at.c1 * N, edge + p.kb_e + at.c1 * N, anew);
+  }
+}
+
+template <typename T, int MODE>
+__global__ __launch_bounds__(256) void paged_append(AppendParams p, Shape sh) {
+  constexpr int N = Elem<T>::N;
+  if (block_x() >= sh.first) {
+    append_run<T, MODE>(p, sh, block_x() - sh.first);
+    return;
+  }
+  const int item = block_x() * 256 + thread_x();
+  const int rest = quot(item, sh.by_units.m, sh.by_units.s), u = item - rest * sh.units;
+  const int token = quot(rest, sh.by_heads.m, sh.by_heads.s);
+  int head = rest - token * sh.heads;
+  const int b = quot(token, sh.by_s.m, sh.by_s.s), i = token - b * p.S;
+  if (b >= p.B) return;
+  const int kind = head >= sh.q_at ? 2 : head >= sh.v_at ? 1 : 0;  // Q, V, K
+  head -= kind == 2 ? sh.q_at : kind == 1 ? sh.v_at : 0;
+  const T* row = kind == 0   ? (const T*)p.k + b * p.k_b + head * p.k_h + i * p.k_s
+                 : kind == 1 ? (const T*)p.v + b * p.v_b + head * p.v_h + i * p.v_s
+                             : (const T*)p.q + b * p.q_b + head * p.q_h + i * p.q_s;
+  Unit<T, MODE> w(u, sh);
+  w.load(row);
+  const int len = seq_len(p.map, b), n = seq_new(p.map, b, p.S, len);
+  const bool fresh = i < n;
+  if (!fresh && kind != 2) return;
+  const int pos = fresh ? len - n + i : 0;
+  const int col = quot(pos, sh.by_ps.m, sh.by_ps.s), slot = pos - col * p.map.page_size;
+  const int page = fresh ? page_at(p.map, b, col) : -1;
+  bool ok = page >= 0;
+  if constexpr (MODE != kCopy) {
+    const int a = p.positions ? p.positions[token] : pos;
+    ok = ok && a >= 0 && a < p.rows;
+    if (kind != 1 && ok) w.rotate(row, p, p.cos + a * p.rot_s, p.sin + a * p.rot_s);
+  }
+  if (kind == 2) {
+    if (!fresh) w.fill((u32x4){0u, 0u, 0u, 0u});
+    else if (!ok) w.fill(Elem<T>::nan());
+    w.store((T*)p.q_out + b * p.o_b + head * p.o_h + i * p.o_s);
+    return;
+  }
+  if (!ok) return;
+  w.store(kind == 0 ? (T*)p.k_pages + page * p.kp_p + head * p.kp_h + slot * p.kp_s
+                    : (T*)p.v_pages + page * p.vp_p + head * p.vp_h + slot * p.vp_s);
+  if (kind == 0 && p.bounds) {  // one token a call: its page's bounds are this unit's alone
+    T* edge = (T*)p.bounds + page * p.kb_p + head * p.kb_h;
+    Range<T> r;
+    r.take(w.x0);
+    r.store(edge + w.c0 * N, edge + p.kb_e + w.c0 * N, slot == 0);
+    if constexpr (MODE == kHalf) {
+      if (w.c1 >= 0) {
+        Range<T> z;
+        z.take(w.x1);
+        z.store(edge + w.c1 * N, edge + p.kb_e + w.c1 * N, slot == 0);
+      }
+    }
+  }
 }
 
 template <typename T>
-__global__ __launch_bounds__(64) void paged_append(AppendParams p) {
+hipError_t launch(const AppendParams& p, hipStream_t s) {
   constexpr int N = Elem<T>::N;
-  const int lane = threadIdx.x, run = blockIdx.x, b = blockIdx.z;
-  int head = blockIdx.y;
-  const int kind = head < p.Hkv ? 0 : head < 2 * p.Hkv ? 1 : 2;  // K, V, Q
-  head -= kind * p.Hkv;
-  const int len = seq_len(p.map, b), n = seq_new(p.map, b, p.S, len);
-  const int pos0 = len - n, ps = p.map.page_size;
-  const int64_t col = (int64_t)(pos0 / ps) + run;
-  const int64_t start = col * ps - pos0;  // the page's slot 0 as a column
-  const int last = kind == 2 ? p.S : n;
-  if (start >= last) return;
-  const int i0 = start > 0 ? (int)start : 0, i1 = start + ps < last ? (int)(start + ps) : last;
-  const int page = page_at(p.map, b, col);
-  const int C = p.D / N, TL = 64 / C;  // chunks of a row, tokens at a time
-  const int t = lane / C, c = lane - t * C;
-  const bool on = t < TL;
-
-  const T* src = kind == 0   ? (const T*)p.k + b * p.k_b + head * p.k_h
-                 : kind == 1 ? (const T*)p.v + b * p.v_b + head * p.v_h
-                             : (const T*)p.q + b * p.q_b + head * p.q_h;
-  const int64_t src_s = kind == 0 ? p.k_s : kind == 1 ? p.v_s : p.q_s;
-  T* dst = kind == 0   ? (T*)p.k_pages + max(page, 0) * p.kp_p + head * p.kp_h
-           : kind == 1 ? (T*)p.v_pages + max(page, 0) * p.vp_p + head * p.vp_h
-                       : (T*)p.q_out + b * p.o_b + head * p.o_h;
-  const int64_t dst_s = kind == 0 ? p.kp_s : kind == 1 ? p.vp_s : p.o_s;
-  const bool edges = kind == 0 && p.bounds != nullptr && page >= 0;
-  float lo[N], hi[N];
-#pragma unroll
-  for (int e = 0; e < N; ++e) {
-    lo[e] = INFINITY;
-    hi[e] = -INFINITY;
-  }
-  if (on) {
-    for (int i = i0 + t; i < i1; i += TL) {
-      const T* row = src + i * src_s;
-      if (i >= n) {  // a padding column of Q
-        *(u32x4*)(dst + i * dst_s + c * N) = (u32x4){0u, 0u, 0u, 0u};
-        continue;
-      }
-      const int at = p.positions ? p.positions[(int64_t)b * p.S + i] : pos0 + i;
-      const bool ok = page >= 0 && (p.rot == 0 || (at >= 0 && at < p.rows));
-      u32x4 w = Elem<T>::nan();
-      if (ok) w = kind == 1 || p.rot == 0 ? *(const u32x4*)(row + c * N)
-                                          : rotated<T>(row, c, p, p.cos + at * p.rot_s, p.sin + at * p.rot_s);
-      if (ok || kind == 2) *(u32x4*)(dst + (kind == 2 ? i : i - start) * dst_s + c * N) = w;
-      if (edges && ok) {
-#pragma unroll
-        for (int e = 0; e < N; ++e) {
-          const float x = Elem<T>::get(w, e);
-          lo[e] = fminf(lo[e], x);
-          hi[e] = fmaxf(hi[e], x);
-        }
-      }
-    }
-  }
-  if (!edges) return;
-  // the token lanes' bounds meet in token lane 0
-  float l0[N], h0[N];
-#pragma unroll
-  for (int e = 0; e < N; ++e) {
-    l0[e] = lo[e];
-    h0[e] = hi[e];
-    for (int s = 1; s < TL; ++s) {
-      l0[e] = fminf(l0[e], __shfl(lo[e], (s * C + lane) & 63));
-      h0[e] = fmaxf(h0[e], __shfl(hi[e], (s * C + lane) & 63));
-    }
-  }
-  if (t != 0) return;
-  T* edge = (T*)p.bounds + page * p.kb_p + head * p.kb_h + c * N;
-  if (start < 0) {  // the page held keys before
-    const u32x4 a = *(const u32x4*)edge, z = *(const u32x4*)(edge + p.kb_e);
-#pragma unroll
-    for (int e = 0; e < N; ++e) {
-      l0[e] = fminf(l0[e], Elem<T>::get(a, e));
-      h0[e] = fmaxf(h0[e], Elem<T>::get(z, e));
-    }
-  }
-  *(u32x4*)edge = Elem<T>::put(l0);
-  *(u32x4*)(edge + p.kb_e) = Elem<T>::put(h0);
+  // chunks turn whole where halves, or the rotated part, are whole chunks and
+  // the tables' rows are read in 16 bytes
+  const int h = p.rot / 2;
+  const bool tables = (((uintptr_t)p.cos | (uintptr_t)p.sin) & 15u) == 0 && p.rot_s % 4 == 0;
+  const Mode mode = p.rot == 0                                               ? kCopy
+                    : tables && !p.interleaved && h % N == 0                ? kHalf
+                    : tables && p.interleaved && p.rot % N == 0             ? kSide
+                                                                            : kAny;
+  Shape sh;
+  const int chunks = p.D / N, ps = p.map.page_size;
+  sh.pairs = mode == kHalf ? h / N : 0;
+  sh.units = chunks - sh.pairs;
+  const bool by_runs = p.bounds && p.S > 1;
+  sh.v_at = by_runs ? 0 : p.Hkv;
+  sh.q_at = sh.v_at + p.Hkv;
+  sh.heads = sh.q_at + p.H;
+  const int64_t items = (int64_t)p.B * p.S * sh.heads * sh.units;
+  sh.first = (int)((items + 255) / 256);
+  // pages that S tokens beginning in any slot touch at most
+  sh.runs = by_runs ? (p.S - 1 + ps - 1) / ps + 1 : 1;
+  const int64_t second = by_runs ? (int64_t)p.B * ((p.Hkv + 3) / 4) * sh.runs : 0;
+  sh.by_units = div_by(sh.units);
+  sh.by_heads = div_by(sh.heads);
+  sh.by_s = div_by(p.S);
+  sh.by_ps = div_by(ps);
+  sh.by_runs = div_by(sh.runs);
+  sh.by_groups = div_by((p.Hkv + 3) / 4);
+  const dim3 grid((unsigned)(sh.first + second)), block(256);
+  if (mode == kCopy) hipLaunchKernelGGL((paged_append<T, kCopy>), grid, block, 0, s, p, sh);
+  else if (mode == kHalf) hipLaunchKernelGGL((paged_append<T, kHalf>), grid, block, 0, s, p, sh);
+  else if (mode == kSide) hipLaunchKernelGGL((paged_append<T, kSide>), grid, block, 0, s, p, sh);
+  else hipLaunchKernelGGL((paged_append<T, kAny>), grid, block, 0, s, p, sh);
+  return hipGetLastError();
 }
 
 }  // namespace
 
 hipError_t launch_paged_append(const AppendParams& p, int dtype, hipStream_t s) {
-  const int ps = p.map.page_size;
-  // pages that S tokens beginning in any slot touch at most
-  const int64_t runs = ((int64_t)p.S - 1 + ps - 1) / ps + 1;
-  const dim3 grid((unsigned)runs, 2 * p.Hkv + p.H, p.B), block(64);
-  if (dtype == 0) hipLaunchKernelGGL(paged_append<_Float16>, grid, block, 0, s, p);
-  else if (dtype == 1) hipLaunchKernelGGL(paged_append<__bf16>, grid, block, 0, s, p);
-  else hipLaunchKernelGGL(paged_append<float>, grid, block, 0, s, p);
-  return hipGetLastError();
+  if (dtype == 0) return launch<_Float16>(p, s);
+  if (dtype == 1) return launch<__bf16>(p, s);
+  return launch<float>(p, s);
 }
 
 }  // namespace cmpext3

@@ -116,15 +116,6 @@ __device__ __forceinline__ void lds_dma16_fresh(const u32x4& rs, uint32_t lds_by
   asm volatile("s_nop 4\n\tbuffer_load_dwordx4 %0, %1, 0 offen lds" ::"v"(voff), "s"(rs), "{m0}"(lds_byte) : "memory");
 }
 
-// n / d for 0 <= n < 2^31 as a product: s = ceil(log2 d), m = floor(2^(31+s) / d)
-// + 1 exceeds the quotient's scale by less than 2^s / 2^(31+s), too little to
-// reach the next whole number.
-struct Div {
-  uint32_t m;
-  int s;
-};
-__device__ __forceinline__ int quot(int n, uint32_t m, int s) { return (int)(__umulhi((uint32_t)n << 1, m) >> s); }
-
 struct AttnArgs {
   const int32_t *lens, *news, *table, *selected;
   int64_t t_str;
@@ -805,12 +796,6 @@ int workgroups(int dtype, int B, int H, int Hkv, int S, int D, int page_size, in
   return most < n ? (int)most : n;
 }
 
-Div div_by(int d) {
-  int s = 0;
-  while ((1ll << s) < d) ++s;
-  return {(uint32_t)((1ull << (31 + s)) / (uint32_t)d + 1), s};
-}
-
 template <typename T, int DK>
 hipError_t launch_dk(const AttnArgs& a, int wgs, hipStream_t s) {
   const dim3 grid(wgs), block(pg_waves(DK * sizeof(T)) * 64);
@@ -838,7 +823,7 @@ size_t paged_attn_workspace(int dtype, int B, int H, int Hkv, int S, int D, int 
   // tiles are counted in 32 bits: a table for more is read in whole units
   const int64_t cols = n_selected > 0 ? n_selected : width;
   const int64_t units = (int64_t)B * Hkv * ((H / Hkv * S + kRows - 1) / kRows);
-  if (n <= 1 || units * (cols * ((page_size + kTile - 1) / kTile) + kSetup) > INT32_MAX / 2) return 0;
+  if (n <= 1 || width == 0 || units * (cols * ((page_size + kTile - 1) / kTile) + kSetup) > INT32_MAX / 2) return 0;
   return kExchangeCounterBytes + (size_t)n * 2 * kRows * (bucket(dtype, D) / 4 + 1) * sizeof(f32x4);
 }
 
