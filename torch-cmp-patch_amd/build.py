@@ -33,7 +33,8 @@ HIP_SOURCES = ["attn_fwd_mfma16.hip", "attn_fwd_pipe16_f16.hip", "attn_fwd_pipe1
                "attn_fwd_pipe16_bf16.hip", "attn_fwd_plan16.hip", "attn_fwd_pipe16w.hip", "attn_fwd_pipe16wm.hip", "attn_fwd_pipe16b.hip",
                "attn_fwd_mask_bits.hip", "attn_fwd_short16.hip", "attn_fwd_mfma32.hip",
                "attn_fwd_decode16.hip", "attn_bwd16.hip", "attn_bwd32.hip", "attn_abi.cpp",
-               "paged_append.hip", "paged_attn.hip", "paged_select.hip", "paged_abi.cpp"]
+               "paged_append.hip", "paged_attn.hip", "paged_attn_f16.hip",
+               "paged_attn_bf16.hip", "paged_attn_f32.hip", "paged_select.hip", "paged_abi.cpp"]
 NATIVE_SOURCES = ["main.cpp", "paged_binding.cpp"]
 HIP_FLAGS = [
     f"--offload-arch={ARCH}", "-O3", "-std=c++17", "-fPIC", "-Wall",
@@ -56,7 +57,9 @@ FILE_FLAGS_DROP = {"attn_fwd_pipe16_f16.hip": {"-mno-amdgpu-ieee", "-fno-honor-n
                    "attn_fwd_pipe16b.hip": {"-mno-amdgpu-ieee", "-fno-honor-nans"},
                    # the paged kernels' bounds, orders and error rows rely on NaN
                    "paged_append.hip": {"-mno-amdgpu-ieee", "-fno-honor-nans"},
-                   "paged_attn.hip": {"-mno-amdgpu-ieee", "-fno-honor-nans"},
+                   "paged_attn_f16.hip": {"-mno-amdgpu-ieee", "-fno-honor-nans"},
+                   "paged_attn_bf16.hip": {"-mno-amdgpu-ieee", "-fno-honor-nans"},
+                   "paged_attn_f32.hip": {"-mno-amdgpu-ieee", "-fno-honor-nans"},
                    "paged_select.hip": {"-mno-amdgpu-ieee", "-fno-honor-nans"}}
 
 LIB_NAME = "libcmpext3_attn.so"

@@ -1,0 +1,6 @@
+// fp16 instantiations of the paged attention kernel.
+#include "paged_attn.h"
+
+namespace cmpext3 {
+hipError_t launch_paged_attn_f16(const AttnArgs& a, int wgs, hipStream_t s) { return launch_type<_Float16>(a, wgs, s); }
+}  // namespace cmpext3
