@@ -100,7 +100,7 @@ int cmpext3_paged_append(const void* k, const void* v, const void* q, void* q_ou
   if (q && q == q_out) return CMPEXT3_E_INVALID;
   // 32-bit item numbers, and a grid of less than 2^32 threads
   if ((int64_t)B * S * (2 * (int64_t)H_kv + (q ? H : 0)) * (D * es / 16) > INT32_MAX / 2 ||
-      (key_bounds && (int64_t)B * (H_kv / 4 + 1) * (S / page_size + 2) > (1 << 23)))
+      (key_bounds && (int64_t)B * H_kv * (S / page_size + 2) > (1 << 23)))
     return CMPEXT3_E_TOO_LARGE;
   if (((uintptr_t)new_lens | (uintptr_t)positions | (uintptr_t)cos | (uintptr_t)sin) & 3u) return CMPEXT3_E_ALIGN;
   if (cos && (rot < 2 || rot % 2 != 0 || rot > D || table_rows < 1 || (table_rows > 1 && rot_stride < 0)))

@@ -73,7 +73,8 @@ enum Mode {
 struct Shape {
   int units, pairs;  // units of a row; the first `pairs` of them are two chunks, `pairs` apart
   int heads;         // heads of a token in the first section: V and Q, and K where it takes no runs
-  int runs;          // workgroups of the second section per (sequence, 4 heads): 0 without it
+  int runs;          // second section: runs per (sequence, head)
+  int waves;         // waves of a run, 1 or 4
   int first;         // workgroups of the first section
   int q_at, v_at;    // where V's and Q's heads begin in a token's
   Div by_units, by_heads, by_s, by_ps, by_runs, by_groups;
@@ -171,7 +172,7 @@ template <typename T>
 struct Range {
   static constexpr int N = Elem<T>::N;
   float lo[N], hi[N];
-  __device__ __forceinline__ Range() {
+  __device__ __forceinline__ void clear() {
 #pragma unroll
     for (int e = 0; e < N; ++e) {
       lo[e] = INFINITY;
@@ -183,6 +184,13 @@ struct Range {
     for (int e = 0; e < N; ++e) {
       lo[e] = fminf(lo[e], Elem<T>::get(w, e));
       hi[e] = fmaxf(hi[e], Elem<T>::get(w, e));
+    }
+  }
+  __device__ __forceinline__ void take(const Range& o) {
+#pragma unroll
+    for (int e = 0; e < N; ++e) {
+      lo[e] = fminf(lo[e], o.lo[e]);
+      hi[e] = fmaxf(hi[e], o.hi[e]);
     }
   }
   // over the lanes of the same unit, `units` apart, `n` of them, into the first
@@ -217,8 +225,9 @@ __device__ __forceinline__ void append_run(const AppendParams& p, const Shape& s
   constexpr int N = Elem<T>::N;
   const int lane = thread_x() & 63, wave = __builtin_amdgcn_readfirstlane(thread_x() >> 6);
   const int rest = quot(wg, sh.by_runs.m, sh.by_runs.s), run = wg - rest * sh.runs;
-  const int groups = (p.Hkv + 3) / 4;
-  const int b = quot(rest, sh.by_groups.m, sh.by_groups.s), head = (rest - b * groups) * 4 + wave;
+  const int heads = 4 / sh.waves, groups = (p.Hkv + heads - 1) / heads;  // a workgroup's heads
+  const int b = quot(rest, sh.by_groups.m, sh.by_groups.s);
+  const int head = (rest - b * groups) * heads + (sh.waves == 1 ? wave : 0);
   if (head >= p.Hkv) return;
   const int len = seq_len(p.map, b), n = seq_new(p.map, b, p.S, len);
   const int pos0 = len - n, ps = p.map.page_size;
@@ -233,10 +242,12 @@ __device__ __forceinline__ void append_run(const AppendParams& p, const Shape& s
   T* dst = (T*)p.k_pages + page * p.kp_p + head * p.kp_h;
   const Unit<T, MODE> at(u, sh);
   Range<T> r0, r1;
+  r0.clear();
+  r1.clear();
   bool some = false;
   if (t < TL) {
 #pragma unroll 2
-    for (int i = i0 + t; i < i1; i += TL) {
+    for (int i = i0 + t + (sh.waves == 1 ? 0 : wave * TL); i < i1; i += TL * sh.waves) {
       const T* row = src + i * p.k_s;
       Unit<T, MODE> w = at;
       w.load(row);
@@ -254,9 +265,27 @@ __device__ __forceinline__ void append_run(const AppendParams& p, const Shape& s
       }
     }
   }
-  if (!__builtin_amdgcn_ballot_w64(some)) return;
+  if (sh.waves == 1 && !__builtin_amdgcn_ballot_w64(some)) return;
   r0.join(lane, t, TL, sh.units);
   if constexpr (MODE == kHalf) r1.join(lane, t, TL, sh.units);
+  if (sh.waves > 1) {  // the four waves' bounds meet in the first
+    __shared__ Range<T> far[3][2][64];
+    __shared__ int any;
+    if (thread_x() == 0) any = 0;
+    __syncthreads();
+    if (some) any = 1;
+    if (wave > 0 && t == 0) {
+      far[wave - 1][0][lane] = r0;
+      if constexpr (MODE == kHalf) far[wave - 1][1][lane] = r1;
+    }
+    __syncthreads();
+    if (wave > 0 || !any) return;
+    if (t == 0)
+      for (int w = 0; w < 3; ++w) {
+        r0.take(far[w][0][lane]);
+        if constexpr (MODE == kHalf) r1.take(far[w][1][lane]);
+      }
+  }
   if (t != 0) return;
   const bool anew = start >= 0;  // the page begins with a new token
   T* edge = (T*)p.bounds + page * p.kb_p + head * p.kb_h;
@@ -310,11 +339,13 @@ __global__ __launch_bounds__(256) void paged_append(AppendParams p, Shape sh) {
   if (kind == 0 && p.bounds) {  // one token a call: its page's bounds are this unit's alone
     T* edge = (T*)p.bounds + page * p.kb_p + head * p.kb_h;
     Range<T> r;
+    r.clear();
     r.take(w.x0);
     r.store(edge + w.c0 * N, edge + p.kb_e + w.c0 * N, slot == 0);
     if constexpr (MODE == kHalf) {
       if (w.c1 >= 0) {
         Range<T> z;
+        z.clear();
         z.take(w.x1);
         z.store(edge + w.c1 * N, edge + p.kb_e + w.c1 * N, slot == 0);
       }
@@ -345,13 +376,16 @@ hipError_t launch(const AppendParams& p, hipStream_t s) {
   sh.first = (int)((items + 255) / 256);
   // pages that S tokens beginning in any slot touch at most
   sh.runs = by_runs ? (p.S - 1 + ps - 1) / ps + 1 : 1;
-  const int64_t second = by_runs ? (int64_t)p.B * ((p.Hkv + 3) / 4) * sh.runs : 0;
+  // a run of more tokens than a wave takes in two steps goes to four waves
+  sh.waves = by_runs && (ps < p.S ? ps : p.S) * sh.units > 2 * 64 ? 4 : 1;
+  const int heads = 4 / sh.waves, groups = (p.Hkv + heads - 1) / heads;
+  const int64_t second = by_runs ? (int64_t)p.B * groups * sh.runs : 0;
   sh.by_units = div_by(sh.units);
   sh.by_heads = div_by(sh.heads);
   sh.by_s = div_by(p.S);
   sh.by_ps = div_by(ps);
   sh.by_runs = div_by(sh.runs);
-  sh.by_groups = div_by((p.Hkv + 3) / 4);
+  sh.by_groups = div_by(groups);
   const dim3 grid((unsigned)(sh.first + second)), block(256);
   if (mode == kCopy) hipLaunchKernelGGL((paged_append<T, kCopy>), grid, block, 0, s, p, sh);
   else if (mode == kHalf) hipLaunchKernelGGL((paged_append<T, kHalf>), grid, block, 0, s, p, sh);

@@ -78,7 +78,7 @@ constexpr int kTile = 16;        // slots of a tile
 constexpr int kMaxWgs = 1024;    // workgroups of a launch at most (counters: one each)
 constexpr int kMinTiles = 16;    // tiles of a workgroup's share at least
 constexpr int kSetup = 6;        // what a unit costs beside its tiles, in tiles
-constexpr int kWhole = 32;       // tiles of a unit that is never split
+constexpr int kShortCut = 40;    // tiles of a part up to which units are cut by themselves
 constexpr int kLongShare = 48;   // tiles of a share from which one workgroup a CU is enough
 constexpr int kJoin = 8;         // parts joined at once
 
@@ -206,6 +206,10 @@ __global__ __launch_bounds__(pg_waves(DK * sizeof(T)) * 64, pg_waves(DK * sizeof
   constexpr int DQ = DK / 4;            // float4 vectors of an output row
   constexpr int MOS = DK + 4;           // row stride (floats) of the waves' states
   constexpr int ROWS = NR * kRows;      // query rows of a unit at most
+  // tiles of a unit that is never split: a join costs about that many (fp32
+  // products take longer).  bf16 [1,16/8,1,300,128] 7.7 us whole, 10.7 in parts;
+  // fp32 [2,20/5,2,500,128] 18.7 us with 32 here, 12.2 with 16.
+  constexpr int kWhole = F32 ? 16 : 32;
   constexpr int RING = NW * NS * STAGE;
   static_assert(BLK % 1024 == 0 && NC % 4 == 0 && (!F32 || DK % 64 == 0), "head dim bucket");
   static_assert(NS >= 1 && IPT * (NS - 1) <= 63, "vmcnt range");
@@ -265,7 +269,11 @@ __global__ __launch_bounds__(pg_waves(DK * sizeof(T)) * 64, pg_waves(DK * sizeof
   bool idle = true;     // a sequence has no tiles
   int depth = NS;       // stages in use
   Seq held = {0, 0, 0};  // B <= 64: lane b's is sequence b
+  int cut = 0;          // > 0: units are cut by themselves
   auto weight_of = [](int tiles) { return tiles > 0 ? tiles + kSetup : 0; };
+  auto parts_of = [&](int tiles, int cut) {
+    return tiles == 0 ? 0 : tiles <= kWhole ? 1 : (int)((uint32_t)(weight_of(tiles) + cut - 1) / (uint32_t)cut);
+  };
   // sequence i of the batch, the same for every lane
   auto seq_at = [&](int i) {
     Seq s = held;
@@ -300,17 +308,34 @@ __global__ __launch_bounds__(pg_waves(DK * sizeof(T)) * 64, pg_waves(DK * sizeof
       const int all = __builtin_amdgcn_readlane(wave_scan(busy), 63);
       idle = all < B;
       // as many shares as workgroups, but of kMinTiles at least, or a unit each
-      int n = min(nwg, max(total / kMinTiles, all * U));
+      const int units = all * U;
+      int n = min(nwg, max(total / kMinTiles, units));
       // Two workgroups a CU, one setting up or joining while the other streams:
       // each with half of its stages, as what waits in the memory's queues
       // delays whatever a set-up needs (ragged fp16 batch 53.4 us with all, 48.7
       // with half).  Where units are long and few, nothing but the sweep counts:
       // one workgroup with all stages (bf16 [16,16/8,4096,128] 54.3 -> 52.0 us).
-      if (n == p->full) {
-        if (all * U < n / 2 && total / (n / 2) >= kLongShare) n /= 2;
-        else depth = (NS + 1) / 2;
+      const bool alone = n == p->full && units < n / 2 && total / (n / 2) >= kLongShare;
+      if (alone) n /= 2;
+      // Short shares: a second segment costs as much as the share itself.  Every
+      // unit is cut by itself, into parts of `cut` at most, a workgroup each.
+      if (per == 1 && !alone && units < nwg) {
+        cut = max(kMinTiles, (int)((uint32_t)total / (uint32_t)(nwg - units)) + 1);
+        if (cut > kShortCut) cut = 0;
       }
-      if (wg < n) {
+      if (cut > 0) {
+        const int own = parts_of(held.tiles, cut), upto = wave_scan(own);
+        const int last = __builtin_amdgcn_readlane(upto, 63) * U;
+        if (2 * last > p->full) depth = (NS + 1) / 2;
+        if (wg < last) {
+          x = wg;
+          hi = wg + 1;
+          const int at = (int)__builtin_ctzll(__builtin_amdgcn_ballot_w64((upto - own) * U <= x && x < upto * U));
+          base = __builtin_amdgcn_readlane(upto - own, at) * U;
+          b = at;
+        }
+      } else if (wg < n) {
+        if (n == p->full) depth = (NS + 1) / 2;
         share = (int)(((uint32_t)total + (uint32_t)n - 1u) / (uint32_t)n);
         x = wg * share;
         hi = min(x + share, total);
@@ -334,7 +359,16 @@ __global__ __launch_bounds__(pg_waves(DK * sizeof(T)) * 64, pg_waves(DK * sizeof
     Seq seq;
     int i, ta = 0, tb, parts = 1, part = 0, w0 = 0;
     const ArgsPtr p = anew(args);
-    if (p->split) {
+    if (cut > 0) {
+      seq = seq_at(b);
+      parts = parts_of(seq.tiles, cut);
+      i = (int)((uint32_t)(x - base) / (uint32_t)parts);
+      part = x - base - i * parts;
+      w0 = wg - part;
+      ta = (int)((uint32_t)(part * seq.tiles) / (uint32_t)parts);
+      tb = (int)((uint32_t)((part + 1) * seq.tiles) / (uint32_t)parts);
+      x = hi;
+    } else if (p->split) {
       const int U = p->U;
       seq = seq_at(b);
       int w = weight_of(seq.tiles);
