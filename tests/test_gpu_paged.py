@@ -128,6 +128,31 @@ def test_infinite_and_low_scores(dtype):
     check_attention(dtype, out, q, c, 1.0)
 
 
+@pytest.mark.parametrize("dtype", ["bf16", "fp16", "fp32"])
+@pytest.mark.parametrize("D,H", [(64, 4), (128, 20), (256, 2)])
+@pytest.mark.parametrize("bad", [float("nan"), float("inf"), float("-inf")])
+def test_values_of_later_tokens_reach_no_earlier_one(dtype, D, H, bad):
+    """A NaN or an infinity in a new token's V is its own row's and the later ones'; padding columns stay zero
+    whatever V holds."""
+    c = Cache(dtype, [37, 70, 100], 2, D, 16)
+    q = c.rows(H, 6)
+    c.vp[c.table[0, 34 // 16].long(), :, 34 % 16, 5] = bad   # token 34: column 3 of 6
+    c.vp[c.table[1, 0].long(), 1, 2, D - 1] = bad            # an old token: every row of its head
+    c.vp[c.table[2, 99 // 16].long(), 0, 99 % 16, 0] = bad   # the last of three
+    new = torch.tensor([6, 4, 3], dtype=torch.int32, device="cuda")
+    out = cmpext3.paged_attention(q, c.kp, c.vp, c.table, c.lens, 0.1, new_lens=new)
+    got = po.f64(out)
+    want, wt, top = po.attention(q, c.kp, c.vp, c.table, c.lens, 0.1, new.cpu())
+    assert np.array_equal(np.isfinite(got), np.isfinite(want))
+    assert np.array_equal(np.isnan(got), np.isnan(want)) and (got[np.isinf(want)] == want[np.isinf(want)]).all()
+    assert (got[1, :, 4:] == 0).all() and (got[2, :, 3:] == 0).all()
+    ok = np.isfinite(want)
+    u = half_step(dtype)
+    rel = 2 * (D + 8) * U32 * top[..., None] + 2 * (100 + 64) * U32 + (0 if dtype == "fp32" else 2 * u)
+    tol = u * np.abs(want[ok]) + (1.01 * rel * wt)[ok] + 2.0 ** -24
+    assert (np.abs(got[ok] - want[ok]) <= tol).all()
+
+
 def test_attention_past_32_bit_offsets():
     """Pages beyond 4 GiB into the pool."""
     P, Hkv, page, D = 40000, 8, 32, 256  # 5.2 GB for K, the same memory for V
@@ -218,6 +243,28 @@ def test_append(case, own_positions):
             if not written[p, 0]:
                 lo, hi = torch.minimum(lo, kb0[p, :, 0].float()), torch.maximum(hi, kb0[p, :, 1].float())
             assert torch.equal(kb[p, :, 0].float(), lo) and torch.equal(kb[p, :, 1].float(), hi)
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "fp16", "fp32"])
+@pytest.mark.parametrize("S,page", [(1, 16), (5, 16), (40, 128)])
+def test_bounds_leave_out_nan_keys(dtype, S, page):
+    c = Cache(dtype, [90, S], 2, 64, page)
+    k = c.rows(2, S)
+    k[:, 0, S // 2] = float("nan")
+    k[1, 1, 0] = float("inf")
+    kb = torch.zeros(c.kp.shape[0], 2, 2, 64, dtype=c.dtype, device="cuda")
+    kb[:, :, 0], kb[:, :, 1] = -0.5, 0.5
+    was = kb.clone()
+    cmpext3.paged_append(k, k, c.kp, c.vp, c.table, c.lens, key_bounds=kb)
+    for b, n in enumerate([90, S]):
+        for p in range((n - S) // page, -(-n // page)):
+            first, last = max(p * page, n - S), min((p + 1) * page, n)
+            x = k[b, :, first - n + S:last - n + S].float().cpu().numpy()
+            lo, hi = np.fmin.reduce(x, axis=1, initial=np.inf), np.fmax.reduce(x, axis=1, initial=-np.inf)
+            page_no = int(c.table[b, p])
+            if first > p * page:
+                lo, hi = np.fmin(lo, po.f64(was[page_no, :, 0])), np.fmax(hi, po.f64(was[page_no, :, 1]))
+            assert np.array_equal(po.f64(kb[page_no, :, 0]), lo) and np.array_equal(po.f64(kb[page_no, :, 1]), hi)
 
 
 def test_append_leaves_out_tokens_without_a_page_or_a_rotation_row():

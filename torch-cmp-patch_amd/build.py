@@ -57,6 +57,7 @@ FILE_FLAGS_DROP = {"attn_fwd_pipe16_f16.hip": {"-mno-amdgpu-ieee", "-fno-honor-n
                    "attn_fwd_pipe16b.hip": {"-mno-amdgpu-ieee", "-fno-honor-nans"},
                    # the paged kernels' bounds, orders and error rows rely on NaN
                    "paged_append.hip": {"-mno-amdgpu-ieee", "-fno-honor-nans"},
+                   "paged_attn.hip": {"-mno-amdgpu-ieee", "-fno-honor-nans"},
                    "paged_attn_f16.hip": {"-mno-amdgpu-ieee", "-fno-honor-nans"},
                    "paged_attn_bf16.hip": {"-mno-amdgpu-ieee", "-fno-honor-nans"},
                    "paged_attn_f32.hip": {"-mno-amdgpu-ieee", "-fno-honor-nans"},

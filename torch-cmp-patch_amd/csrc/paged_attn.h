@@ -23,7 +23,8 @@
 //    for fp16 and bf16, 16x16x4 for fp32), exact online softmax in the exp2
 //    domain with fp32 state.  For fp16 and bf16 a weight enters the second
 //    product in two parts, its value rounded to the tensors' type and the
-//    rounded rest (the matrix units are idle for most of the time anyway).
+//    rounded rest (the matrix units are idle for most of the time anyway), whose
+//    product with an infinity is no number: then the wave sweeps once more.
 //  * End of a segment: the waves' (O, m, l) meet in LDS.  A unit that is one
 //    segment is written out; otherwise each of its workgroups leaves its part
 //    in the workspace and counts itself in, and the last one joins the parts in
@@ -104,7 +105,7 @@ constexpr int pg_lds(int dk, int es) {
 // two; [7,40/5,8,8k..16k,128] 143 with one, 84.9 with two, 92.7 with four and one
 // workgroup a CU.
 constexpr int pg_row_blocks(int rb, int rows) {
-  const int most = rb <= 192 ? 4 : rb <= 384 ? 2 : 1;
+  const int most = rb <= 128 ? 4 : rb <= 256 ? 2 : 1;
   const int n = rows <= kRows ? 1 : rows <= 2 * kRows ? 2 : 4;
   return n < most ? n : most;
 }
@@ -124,6 +125,10 @@ __device__ __forceinline__ int pg_swz(int r, int c, int nc) {
 __device__ __forceinline__ void lds_dma16_fresh(const u32x4& rs, uint32_t lds_byte, int voff) {
   asm volatile("s_nop 4\n\tbuffer_load_dwordx4 %0, %1, 0 offen lds" ::"v"(voff), "s"(rs), "{m0}"(lds_byte) : "memory");
 }
+
+template <bool V> struct Const {
+  static constexpr bool value = V;
+};
 
 struct AttnArgs {
   const int32_t *lens, *news, *table, *selected;
@@ -502,143 +507,202 @@ __global__ __launch_bounds__(pg_waves(DK * sizeof(T)) * 64, pg_waves(DK * sizeof
 
     f32x4 oacc[NR][NDB];
     float m_run[NR], l_run[NR];
-#pragma unroll
-    for (int z = 0; z < NR; ++z) {
-      m_run[z] = -INFINITY;
-      l_run[z] = 0.f;
-#pragma unroll
-      for (int db = 0; db < NDB; ++db) oacc[z][db] = (f32x4){0.f, 0.f, 0.f, 0.f};
-    }
     const float cmul = anew(args)->c;
 
-    take(0);
-    // (position, slots) of the tiles in flight: the lanes move on to the next 64
-    // tiles when the first of those is issued, up to NS tiles ahead
-    int pos_q[NS], slots_q[NS];
-#pragma unroll
-    for (int j = 0; j < NS; ++j) {
-      pos_q[j] = slots_q[j] = 0;
-      if (j < mine && j < depth) {
-        pos_q[j] = __builtin_amdgcn_readlane(pos0, j);
-        slots_q[j] = __builtin_amdgcn_readlane(slots0, j);
-        issue(j);
-      }
-    }
-
-    for (int j = 0; j < mine; ++j) {
-      const int behind = min(depth - 1, mine - 1 - j);
-      if (NS > 3 && behind == 3) wait_vmcnt<(NS > 3 ? 3 * IPT : 0)>();
-      else if (NS > 2 && behind == 2) wait_vmcnt<(NS > 2 ? 2 * IPT : 0)>();
-      else if (NS > 1 && behind == 1) wait_vmcnt<(NS > 1 ? IPT : 0)>();
-      else wait_vmcnt<0>();
-      const unsigned char* st = lds + (wave * NS + j % NS) * STAGE;
-      const int pos = pos_q[0], slots = slots_q[0];
-#pragma unroll
-      for (int q = 0; q + 1 < NS; ++q) {
-        pos_q[q] = pos_q[q + 1];
-        slots_q[q] = slots_q[q + 1];
-      }
-
-      f32x4 s[NR];
-#pragma unroll
-      for (int z = 0; z < NR; ++z) s[z] = (f32x4){0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-      for (int ks = 0; ks < KS; ++ks) {
-        const u32x4 kk = *(const u32x4*)(st + kro[ks]);
-#pragma unroll
-        for (int z = 0; z < NR; ++z) {
-          if constexpr (F32) {
-#pragma unroll
-            for (int e = 0; e < 4; ++e)
-              s[z] = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(kk[e]), __uint_as_float(qf[z][ks][e]), s[z], 0, 0, 0);
-          } else {
-            s[z] = Mma<T>::qk(kk, qf[z][ks], s[z]);
-          }
-        }
-      }
-      float pe[NR][4];
-      u32x2 pb[NR], pl[NR];  // fp16, bf16: rounded weights, and what the rounding left
+    // A sum that is no number: an infinity in V met the rest of its weight's
+    // rounding, or a value that some rows do not see met their weight of 0.  The
+    // wave sweeps its tiles once more, carefully.
+    auto sweep = [&](auto kind) {
+      constexpr bool careful = decltype(kind)::value;
 #pragma unroll
       for (int z = 0; z < NR; ++z) {
-        float xs[4];
+        m_run[z] = -INFINITY;
+        l_run[z] = 0.f;
 #pragma unroll
-        for (int e = 0; e < 4; ++e) xs[e] = s[z][e] * cmul;
-        if (slots < kTile || pos + kTile > sure) {
+        for (int db = 0; db < NDB; ++db) oacc[z][db] = (f32x4){0.f, 0.f, 0.f, 0.f};
+      }
+      take(0);
+      // (position, slots) of the tiles in flight: the lanes move on to the next 64
+      // tiles when the first of those is issued, up to NS tiles ahead
+      int pos_q[NS], slots_q[NS];
 #pragma unroll
-          for (int e = 0; e < 4; ++e)
-            if (4 * g + e >= slots || pos + 4 * g + e >= limit[z]) xs[e] = -INFINITY;
-        }
-        const float mt = rows_max(fmaxf(fmaxf(xs[0], xs[1]), fmaxf(xs[2], xs[3])));
-        if (__builtin_amdgcn_ballot_w64(mt > m_run[z])) {  // some row's maximum rises
-          const float m_new = fmaxf(m_run[z], mt);
-          const float alpha = weight(m_run[z], m_new);
-          m_run[z] = m_new;
-          l_run[z] *= alpha;
-#pragma unroll
-          for (int db = 0; db < NDB; ++db) oacc[z][db] *= alpha;
-        }
-        const float m_sub = m_run[z] == -INFINITY ? 0.f : m_run[z];
-#pragma unroll
-        for (int e = 0; e < 4; ++e) pe[z][e] = fast_exp2(xs[e] - m_sub);
-        l_run[z] += (pe[z][0] + pe[z][1]) + (pe[z][2] + pe[z][3]);
-        if constexpr (!F32) {
-          pb[z][0] = Mma<T>::pack(pe[z][0], pe[z][1]);
-          pb[z][1] = Mma<T>::pack(pe[z][2], pe[z][3]);
-          pl[z][0] = Mma<T>::rest(pb[z][0], pe[z][0], pe[z][1]);
-          pl[z][1] = Mma<T>::rest(pb[z][1], pe[z][2], pe[z][3]);
+      for (int j = 0; j < NS; ++j) {
+        pos_q[j] = slots_q[j] = 0;
+        if (j < mine && j < depth) {
+          pos_q[j] = __builtin_amdgcn_readlane(pos0, j);
+          slots_q[j] = __builtin_amdgcn_readlane(slots0, j);
+          issue(j);
         }
       }
-      const unsigned char* vs = st + BLK;
-      if constexpr (F32) {
-        // 64 columns at a time: MFMA j takes columns 4 m + j (a lane's 16-byte
-        // read is one slot's chunk, an element for each of the four)
+
+      for (int j = 0; j < mine; ++j) {
+        const int behind = min(depth - 1, mine - 1 - j);
+        if (NS > 3 && behind == 3) wait_vmcnt<(NS > 3 ? 3 * IPT : 0)>();
+        else if (NS > 2 && behind == 2) wait_vmcnt<(NS > 2 ? 2 * IPT : 0)>();
+        else if (NS > 1 && behind == 1) wait_vmcnt<(NS > 1 ? IPT : 0)>();
+        else wait_vmcnt<0>();
+        const unsigned char* st = lds + (wave * NS + j % NS) * STAGE;
+        const int pos = pos_q[0], slots = slots_q[0];
 #pragma unroll
-        for (int db = 0; db < NDB; db += 4) {
-#pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            const int r = 4 * g + e;
-            const u32x4 v = *(const u32x4*)(vs + r * RB + 16 * pg_swz(r, 4 * db + c, NC));
-#pragma unroll
-            for (int z = 0; z < NR; ++z)
-#pragma unroll
-              for (int q = 0; q < 4; ++q)
-                oacc[z][db + q] =
-                    __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(v[q]), pe[z][e], oacc[z][db + q], 0, 0, 0);
-          }
+        for (int q = 0; q + 1 < NS; ++q) {
+          pos_q[q] = pos_q[q + 1];
+          slots_q[q] = slots_q[q + 1];
         }
-      } else {
-        // 16 lanes of group g read slots 4g .. 4g+3 x 16 columns, transposed:
-        // lane c receives column 16 db + c of the four
-        const int r = 4 * g + (c >> 2), ch = (c & 3) >> 1;
+
+        f32x4 s[NR];
 #pragma unroll
-        for (int db = 0; db < NDB; ++db) {
-          typedef __attribute__((address_space(3))) i16x4p lds_i16x4;
-          const unsigned char* at = vs + r * RB + 16 * pg_swz(r, 2 * db + ch, NC) + 8 * (c & 1);
-          const i16x4p v = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_i16x4*)at);
+        for (int z = 0; z < NR; ++z) s[z] = (f32x4){0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int ks = 0; ks < KS; ++ks) {
+          const u32x4 kk = *(const u32x4*)(st + kro[ks]);
 #pragma unroll
           for (int z = 0; z < NR; ++z) {
-            oacc[z][db] = Mma<T>::pv(__builtin_bit_cast(u32x2, v), pb[z], oacc[z][db]);
-            oacc[z][db] = Mma<T>::pv(__builtin_bit_cast(u32x2, v), pl[z], oacc[z][db]);
-          }
-        }
-      }
-      const int ahead = j + depth;
-      if (ahead < mine) {
-        if ((ahead & 63) == 0) {
-          look_up(ahead >> 6);
-          take(ahead >> 6);
-        }
+            if constexpr (F32) {
 #pragma unroll
-        for (int q = 0; q < NS; ++q) {
-          if (q == depth - 1) {
-            pos_q[q] = __builtin_amdgcn_readlane(pos0, ahead & 63);
-            slots_q[q] = __builtin_amdgcn_readlane(slots0, ahead & 63);
+              for (int e = 0; e < 4; ++e)
+                s[z] = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(kk[e]), __uint_as_float(qf[z][ks][e]), s[z], 0, 0, 0);
+            } else {
+              s[z] = Mma<T>::qk(kk, qf[z][ks], s[z]);
+            }
           }
         }
-        // this stage's LDS reads have returned before its next tile's loads go out
-        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-        issue(ahead);
+        float pe[NR][4];
+        u32x2 pb[NR], pl[NR];  // fp16, bf16: rounded weights, and what the rounding left
+#pragma unroll
+        for (int z = 0; z < NR; ++z) {
+          float xs[4];
+#pragma unroll
+          for (int e = 0; e < 4; ++e) xs[e] = s[z][e] * cmul;
+          if (slots < kTile || pos + kTile > sure) {
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+              if (4 * g + e >= slots || pos + 4 * g + e >= limit[z]) xs[e] = -INFINITY;
+          }
+          const float mt = rows_max(fmaxf(fmaxf(xs[0], xs[1]), fmaxf(xs[2], xs[3])));
+          if (__builtin_amdgcn_ballot_w64(mt > m_run[z])) {  // some row's maximum rises
+            const float m_new = fmaxf(m_run[z], mt);
+            const float alpha = weight(m_run[z], m_new);
+            m_run[z] = m_new;
+            l_run[z] *= alpha;
+#pragma unroll
+            for (int db = 0; db < NDB; ++db) oacc[z][db] *= alpha;
+          }
+          const float m_sub = m_run[z] == -INFINITY ? 0.f : m_run[z];
+#pragma unroll
+          for (int e = 0; e < 4; ++e) pe[z][e] = fast_exp2(xs[e] - m_sub);
+          l_run[z] += (pe[z][0] + pe[z][1]) + (pe[z][2] + pe[z][3]);
+          if constexpr (!F32) {
+            pb[z][0] = Mma<T>::pack(pe[z][0], pe[z][1]);
+            pb[z][1] = Mma<T>::pack(pe[z][2], pe[z][3]);
+            pl[z][0] = Mma<T>::rest(pb[z][0], pe[z][0], pe[z][1]);
+            pl[z][1] = Mma<T>::rest(pb[z][1], pe[z][2], pe[z][3]);
+          }
+        }
+        const unsigned char* vs = st + BLK;
+        if constexpr (careful) {
+          // rows of one limit at a time, the values behind it blanked
+          const bool cut_off = S > 1 && pos + kTile > len - fresh + 1;
+          for (int i = cut_off ? 0 : fresh - 1; i < fresh; ++i) {
+            const int upto = cut_off ? len - fresh + 1 + i : INT32_MAX;
+#pragma unroll
+            for (int z = 0; z < NR; ++z) {
+              const bool these = !cut_off || limit[z] == upto;
+              if constexpr (F32) {
+#pragma unroll
+                for (int db = 0; db < NDB; db += 4) {
+                  f32x4 t[4] = {};
+#pragma unroll
+                  for (int e = 0; e < 4; ++e) {
+                    const int r = 4 * g + e;
+                    const u32x4 v = *(const u32x4*)(vs + r * RB + 16 * pg_swz(r, 4 * db + c, NC));
+                    const bool in = pos + r < upto;
+#pragma unroll
+                    for (int q = 0; q < 4; ++q)
+                      t[q] = __builtin_amdgcn_mfma_f32_16x16x4f32(in ? __uint_as_float(v[q]) : 0.f, pe[z][e], t[q], 0, 0, 0);
+                  }
+#pragma unroll
+                  for (int q = 0; q < 4; ++q)
+                    if (these) oacc[z][db + q] += t[q];
+                  __builtin_amdgcn_sched_barrier(0);
+                }
+              } else {
+                const int r = 4 * g + (c >> 2), ch = (c & 3) >> 1, left = upto - pos - 4 * g;
+                const uint32_t m0 = (left > 0 ? 0xffffu : 0u) | (left > 1 ? 0xffff0000u : 0u);
+                const uint32_t m1 = (left > 2 ? 0xffffu : 0u) | (left > 3 ? 0xffff0000u : 0u);
+#pragma unroll
+                for (int db = 0; db < NDB; ++db) {
+                  typedef __attribute__((address_space(3))) i16x4p lds_i16x4;
+                  const unsigned char* at = vs + r * RB + 16 * pg_swz(r, 2 * db + ch, NC) + 8 * (c & 1);
+                  const u32x2 v = __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_i16x4*)at)) & (u32x2){m0, m1};
+                  const f32x4 t = Mma<T>::pv(v, pb[z], (f32x4){0.f, 0.f, 0.f, 0.f});
+                  if (these) oacc[z][db] += t;
+                  __builtin_amdgcn_sched_barrier(0);  // one at a time: few registers
+                }
+              }
+            }
+          }
+        } else if constexpr (F32) {
+          // 64 columns at a time: MFMA j takes columns 4 m + j (a lane's 16-byte
+          // read is one slot's chunk, an element for each of the four)
+#pragma unroll
+          for (int db = 0; db < NDB; db += 4) {
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              const int r = 4 * g + e;
+              const u32x4 v = *(const u32x4*)(vs + r * RB + 16 * pg_swz(r, 4 * db + c, NC));
+#pragma unroll
+              for (int z = 0; z < NR; ++z)
+#pragma unroll
+                for (int q = 0; q < 4; ++q)
+                  oacc[z][db + q] =
+                      __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(v[q]), pe[z][e], oacc[z][db + q], 0, 0, 0);
+            }
+          }
+        } else {
+          // 16 lanes of group g read slots 4g .. 4g+3 x 16 columns, transposed:
+          // lane c receives column 16 db + c of the four
+          const int r = 4 * g + (c >> 2), ch = (c & 3) >> 1;
+#pragma unroll
+          for (int db = 0; db < NDB; ++db) {
+            typedef __attribute__((address_space(3))) i16x4p lds_i16x4;
+            const unsigned char* at = vs + r * RB + 16 * pg_swz(r, 2 * db + ch, NC) + 8 * (c & 1);
+            const i16x4p v = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_i16x4*)at);
+#pragma unroll
+            for (int z = 0; z < NR; ++z) {
+              oacc[z][db] = Mma<T>::pv(__builtin_bit_cast(u32x2, v), pb[z], oacc[z][db]);
+              oacc[z][db] = Mma<T>::pv(__builtin_bit_cast(u32x2, v), pl[z], oacc[z][db]);
+            }
+          }
+        }
+        const int ahead = j + depth;
+        if (ahead < mine) {
+          if ((ahead & 63) == 0) {
+            look_up(ahead >> 6);
+            take(ahead >> 6);
+          }
+#pragma unroll
+          for (int q = 0; q < NS; ++q) {
+            if (q == depth - 1) {
+              pos_q[q] = __builtin_amdgcn_readlane(pos0, ahead & 63);
+              slots_q[q] = __builtin_amdgcn_readlane(slots0, ahead & 63);
+            }
+          }
+          // this stage's LDS reads have returned before its next tile's loads go out
+          asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+          issue(ahead);
+        }
       }
+    };
+    sweep(Const<false>());
+    float test = 0.f;
+#pragma unroll
+    for (int z = 0; z < NR; ++z)
+#pragma unroll
+      for (int db = 0; db < NDB; ++db) test += (oacc[z][db][0] + oacc[z][db][1]) + (oacc[z][db][2] + oacc[z][db][3]);
+    if (__builtin_amdgcn_ballot_w64(test != test)) {
+      asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // this wave's last LDS reads
+      look_up(0);
+      sweep(Const<true>());
     }
 
     // ---- end of the segment: outputs, or the workgroup's part of them
@@ -678,6 +742,10 @@ __global__ __launch_bounds__(pg_waves(DK * sizeof(T)) * 64, pg_waves(DK * sizeof
       if (16 * z >= R) break;
       if (z > 0) lds_barrier();  // the last rows have been read
       const float lrow = lost ? __builtin_nanf("") : rows_sum(l_run[z]);
+      if (limit[z] <= 0) {  // sees nothing, whatever V holds
+#pragma unroll
+        for (int db = 0; db < NDB; ++db) oacc[z][db] = (f32x4){0.f, 0.f, 0.f, 0.f};
+      }
 #pragma unroll
       for (int db = 0; db < NDB; ++db) {
         // fp32: accumulators 4 k .. 4 k + 3 hold columns 64 k + 16 g + 4 e + (0 .. 3)
