@@ -6,6 +6,7 @@ import pytest
 import torch
 
 import cmpext3
+from cmpext3 import abi
 from oracle import paged_oracle as po
 from paged_cases import DTYPES, U32, Cache, check_attention, half_step, tables
 
@@ -546,3 +547,56 @@ def test_refusals():
     assert torch.equal(before.view(torch.int16), c.kp.view(torch.int16))
     with torch.no_grad():
         att(q=q.clone().requires_grad_())
+
+
+# dtype, lens, H, Hkv, D, page, S: shares that span units, units cut by themselves, whole units
+SPLITS = [
+    ("bf16", [5000, 70, 0, 2600], 8, 2, 128, 16, 1),
+    ("fp16", [(97 * b) % 3000 for b in range(70)], 8, 4, 64, 16, 1),
+    ("fp32", [3000, 40, 900], 6, 3, 64, 24, 2),
+    ("bf16", [30000], 4, 1, 256, 64, 1),
+    ("bf16", [70000], 2, 1, 8, 16, 1),
+    ("fp16", [2000] * 70, 64, 8, 64, 32, 1),
+    ("bf16", [9000, 9001], 64, 2, 128, 16, 1),
+]
+
+
+@pytest.mark.parametrize("case", SPLITS, ids=lambda c: f"{c[0]}-{max(c[1])}x{len(c[1])}-h{c[2]}.{c[3]}-d{c[4]}")
+def test_whole_and_split_sequences_agree(case):
+    """Without a workspace no sequence is split; a workspace that is too small counts as none; a split leaves its
+    counters at zero and repeats bit for bit.  Both lie within the tolerance of the float64 attention."""
+    dtype, lens, H, Hkv, D, page, S = case
+    c = Cache(dtype, lens, Hkv, D, page)
+    q = c.rows(H, S).contiguous()
+    args = (q, c.kp, c.vp, c.table, c.lens)
+    whole = abi.paged_attention(*args, workspace=None)
+    n = abi.paged_workspace_size(abi.dtype_code(q.dtype), len(lens), H, Hkv, S, D, page, c.table.shape[1])
+    assert n > abi.WORKSPACE_COUNTER_BYTES
+    ws = torch.zeros(n, dtype=torch.uint8, device="cuda")
+    split = abi.paged_attention(*args, workspace=ws)
+    assert not ws[:abi.WORKSPACE_COUNTER_BYTES].any()
+    assert torch.equal(split, abi.paged_attention(*args, workspace=ws))
+    assert not ws[:abi.WORKSPACE_COUNTER_BYTES].any()
+    assert torch.equal(split, cmpext3.paged_attention(*args))
+    assert torch.equal(whole, abi.paged_attention(*args, workspace=ws[:n - 16]))
+    some = [b for b in range(len(lens)) if b < 4]
+    sub = Cache.__new__(Cache)
+    sub.kp, sub.vp, sub.table, sub.lens = c.kp, c.vp, c.table[some], c.lens[some]
+    check_attention(dtype, whole[some], q[some], sub, D ** -0.5)
+    check_attention(dtype, split[some], q[some], sub, D ** -0.5)
+
+
+def test_the_c_entry_points_are_what_the_binding_calls():
+    s = _state(5)
+    kp, vp, kb = s["kp"].clone(), s["vp"].clone(), s["kb"].clone()
+    q = cmpext3.paged_append(s["k"], s["v"], s["kp"], s["vp"], s["table"], s["lens"], query=s["q"], cos=s["cos"],
+                             sin=s["sin"], key_bounds=s["kb"])
+    q2 = abi.paged_append(s["k"], s["v"], kp, vp, s["table"], s["lens"], s["q"], s["cos"], s["sin"], key_bounds=kb)
+    assert torch.equal(q, q2) and torch.equal(kb, s["kb"])
+    assert torch.equal(kp.view(torch.int16), s["kp"].view(torch.int16))
+    sel = cmpext3.paged_select(q, kb, s["table"], s["lens"], 16, 9)
+    assert torch.equal(sel, abi.paged_select(q, kb, s["table"], s["lens"], 16, 9))
+    assert torch.equal(cmpext3.paged_attention(q, kp, vp, s["table"], s["lens"], selected=sel),
+                       abi.paged_attention(q, kp, vp, s["table"], s["lens"], selected=sel))
+    with pytest.raises(RuntimeError, match="code"):
+        abi.paged_attention(q, kp, vp, s["table"], s["lens"], float("nan"))

@@ -1,4 +1,4 @@
-"""ctypes binding of the C ABI in include/cmpext3_attn.h, for torch tensors.
+"""ctypes binding of the C ABI in include/cmpext3_attn.h and include/cmpext3_paged.h, for torch tensors.
 
 This is the FFI stub a host program written in Python would use to call the
 library directly (the torch extension `cmpext3._native` is the other caller).
@@ -367,3 +367,82 @@ def attn_bwd(q, k, v, o, do, lse, scale: Optional[float] = None, causal: bool = 
     if rc != OK:
         raise RuntimeError(f"cmpext3_attn_bwd: {strerror(rc)} (code {rc})")
     return dq, dk, dv
+
+
+# ---- the paged key-value cache (include/cmpext3_paged.h)
+
+
+def _ptr(t):
+    return ctypes.c_void_p(None if t is None else t.data_ptr())
+
+
+def paged_append(key, value, key_pages, value_pages, page_table, seq_lens, query=None, cos=None, sin=None,
+                 positions=None, new_lens=None, interleaved: bool = False, key_bounds=None, stream=None):
+    """cmpext3_paged_append: key, value [B, Hkv, S, D] into their pages, in place; returns the rotated
+    queries (contiguous [B, H, S, D]) or None.  cos and sin contiguous, int tensors int32.  Raises
+    RuntimeError on a non-zero code."""
+    import torch
+    B, Hkv, S, D = key.shape
+    H = Hkv if query is None else query.shape[1]
+    out = None if query is None else torch.empty(query.shape, dtype=query.dtype, device=query.device)
+    none = (ctypes.c_int64 * 3)(0, 0, 0)
+    rc = lib().cmpext3_paged_append(
+        *map(_ptr, (key, value, query, out, key_pages, value_pages, key_bounds)), dtype_code(key.dtype), B, H, Hkv, S, D,
+        key_pages.shape[0], key_pages.shape[2], _strides(key), _strides(value),
+        none if query is None else _strides(query), none if out is None else _strides(out), _strides(key_pages),
+        _strides(value_pages), none if key_bounds is None else _strides(key_bounds), _ptr(page_table),
+        page_table.shape[1], page_table.stride(0), *map(_ptr, (seq_lens, new_lens, positions, cos, sin)),
+        0 if cos is None else cos.shape[0], 0 if cos is None else 2 * cos.shape[1],
+        0 if cos is None else cos.stride(0), int(interleaved), ctypes.c_void_p(_handle(key, stream)))
+    if rc != OK:
+        raise RuntimeError(f"cmpext3_paged_append: {strerror(rc)} (code {rc})")
+    return out
+
+
+def paged_workspace_size(dtype: int, B: int, H: int, H_kv: int, S: int, D: int, page_size: int, table_width: int,
+                         n_selected: int = 0) -> int:
+    """Bytes with which cmpext3_paged_attn splits sequences over workgroups (host only)."""
+    return lib().cmpext3_paged_attn_workspace_size(dtype, B, H, H_kv, S, D, page_size, table_width, n_selected)
+
+
+def paged_attention(query, key_pages, value_pages, page_table, seq_lens, scale: Optional[float] = None, new_lens=None,
+                    selected=None, stream=None, workspace=True):
+    """cmpext3_paged_attn: attention of query [B, H, S, D] over the pages, with this module's workspace
+    of the stream (True), a given byte tensor (its counters zero) or none (None: no sequence is split).
+    Raises RuntimeError on a non-zero code."""
+    import torch
+    B, H, S, D = query.shape
+    P, Hkv, page, _ = key_pages.shape
+    out = torch.empty(query.shape, dtype=query.dtype, device=query.device)
+    handle = _handle(query, stream)
+    n = 0 if selected is None else selected.shape[2]
+    if workspace is True:
+        workspace = workspace_for(query, handle, paged_workspace_size(dtype_code(query.dtype), B, H, Hkv, S, D, page,
+                                                                      page_table.shape[1], n))
+    wp, wb = _space(workspace)
+    rc = lib().cmpext3_paged_attn(
+        *map(_ptr, (query, key_pages, value_pages, out)), dtype_code(query.dtype), B, H, Hkv, S, D, P, page,
+        _strides(query), _strides(key_pages), _strides(value_pages), _strides(out), _ptr(page_table),
+        page_table.shape[1], page_table.stride(0), *map(_ptr, (seq_lens, new_lens, selected)), n,
+        ctypes.c_float(D ** -0.5 if scale is None else scale), ctypes.c_void_p(wp), wb, ctypes.c_void_p(handle))
+    if rc != OK:
+        raise RuntimeError(f"cmpext3_paged_attn: {strerror(rc)} (code {rc})")
+    return out
+
+
+def paged_select(query, key_bounds, page_table, seq_lens, page_size: int, n_selected: int, stream=None):
+    """cmpext3_paged_select: int32 [B, Hkv, n_selected], the pages that query [B, H, 1, D] attends to.
+    Raises RuntimeError on a non-zero code."""
+    import torch
+    B, H, _, D = query.shape
+    P, Hkv = key_bounds.shape[:2]
+    out = torch.empty(B, Hkv, n_selected, dtype=torch.int32, device=query.device)
+    need = lib().cmpext3_paged_select_workspace_size(B, Hkv, page_table.shape[1])
+    ws = torch.empty(need, dtype=torch.uint8, device=query.device) if need else None
+    rc = lib().cmpext3_paged_select(
+        *map(_ptr, (query, key_bounds, out)), dtype_code(query.dtype), B, H, Hkv, D, P, page_size, _strides(query),
+        _strides(key_bounds), _ptr(page_table), page_table.shape[1], page_table.stride(0), _ptr(seq_lens), n_selected,
+        _ptr(ws), need, ctypes.c_void_p(_handle(query, stream)))
+    if rc != OK:
+        raise RuntimeError(f"cmpext3_paged_select: {strerror(rc)} (code {rc})")
+    return out

@@ -137,7 +137,8 @@ struct AttnArgs {
   int nsel, width, ps, tpp;  // tpp: tiles per page
   Div by_ps, by_tpp, by_blocks, by_s;
   int split, exact, full;  // split 0: whole units, dealt out in turn; exact: pages are whole tiles; full: workgroups the CUs hold
-  int G, blocks, rows, num_pages;  // query heads per K/V head, row blocks and rows of a K/V head
+  int G, blocks, rows, num_pages;  // query heads per K/V head, units and rows of a K/V head
+  int slot_rows;                   // rows of a part in the workspace
   const char *k, *v;
   int64_t kp_p, kp_h, vp_p, vp_h;  // bytes
   int ks_b, vs_b, row_b, D;        // bytes of a slot's stride, of a row
@@ -725,12 +726,13 @@ __global__ __launch_bounds__(pg_waves(DK * sizeof(T)) * 64, pg_waves(DK * sizeof
     const ArgsPtr pe_args = anew(args);
     const __amdgpu_buffer_rsrc_t wsr =
         uniform_rsrc(parts > 1 ? (const void*)pe_args->ws : (const void*)pe_args->o,
-                     parts > 1 ? (int64_t)nwg * 2 * ROWS * (DQ + 1) * 16 : 16);
+                     parts > 1 ? (int64_t)nwg * 2 * pe_args->slot_rows * (DQ + 1) * 16 : 16);
     int* const cnt = pe_args->cnt;
+    const int slot_rows = pe_args->slot_rows;
     // slot of part q's row r: a part that begins the unit is its workgroup's
     // last segment, the others are their workgroups' first.  Device-scope (aux
     // 16 = sc1) accesses, coherent across the XCDs' L2s.
-    auto slot = [&](int q, int r, int k) { return ((((w0 + q) * 2 + (q == 0 ? 1 : 0)) * ROWS + r) * (DQ + 1) + k) * 16; };
+    auto slot = [&](int q, int r, int k) { return ((((w0 + q) * 2 + (q == 0 ? 1 : 0)) * slot_rows + r) * (DQ + 1) + k) * 16; };
     auto ld = [&](int off) { return __builtin_bit_cast(f32x4, __builtin_amdgcn_raw_buffer_load_b128(wsr, off, 0, 16)); };
     auto st = [&](int off, f32x4 v) { __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4, v), wsr, off, 0, 16); };
     const bool lost = __builtin_amdgcn_ballot_w64(bad) != 0;  // a page that is none: the unit's rows are NaN

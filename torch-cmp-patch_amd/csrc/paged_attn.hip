@@ -20,6 +20,11 @@ int bucket(int dtype, int D) {
 int unit_rows(int dtype, int D, int rows) {
   return kRows * pg_row_blocks(bucket(dtype, D) * (dtype == 2 ? 4 : 2), rows);
 }
+// Rows of a part in the workspace.
+int slot_rows(int dtype, int D, int rows) {
+  const int n = unit_rows(dtype, D, rows);
+  return rows < n ? rows : n;
+}
 int64_t unit_count(int dtype, int B, int H, int Hkv, int S, int D) {
   const int rows = H / Hkv * S, n = unit_rows(dtype, D, rows);
   return (int64_t)B * Hkv * ((rows + n - 1) / n);
@@ -51,7 +56,7 @@ size_t paged_attn_workspace(int dtype, int B, int H, int Hkv, int S, int D, int 
   const int64_t cols = n_selected > 0 ? n_selected : width;
   const int64_t units = unit_count(dtype, B, H, Hkv, S, D);
   if (n <= 1 || width == 0 || units * (cols * ((page_size + kTile - 1) / kTile) + kSetup) > INT32_MAX / 2) return 0;
-  return kExchangeCounterBytes + (size_t)n * 2 * unit_rows(dtype, D, H / Hkv * S) * (bucket(dtype, D) / 4 + 1) * sizeof(f32x4);
+  return kExchangeCounterBytes + (size_t)n * 2 * slot_rows(dtype, D, H / Hkv * S) * (bucket(dtype, D) / 4 + 1) * sizeof(f32x4);
 }
 
 hipError_t launch_paged_attn(const PagedAttnParams& p, int dtype, hipStream_t s) {
@@ -69,7 +74,7 @@ hipError_t launch_paged_attn(const PagedAttnParams& p, int dtype, hipStream_t s)
   a.by_ps = div_by(ps); a.by_tpp = div_by(tpp); a.by_blocks = div_by(blocks); a.by_s = div_by(p.S);
   a.exact = ps % kTile == 0;
   a.full = full_house(dtype, p.D);
-  a.G = G; a.blocks = blocks; a.rows = G * p.S; a.num_pages = p.map.num_pages;
+  a.G = G; a.blocks = blocks; a.rows = G * p.S; a.slot_rows = slot_rows(dtype, p.D, G * p.S); a.num_pages = p.map.num_pages;
   a.k = (const char*)p.k; a.v = (const char*)p.v;
   a.kp_p = p.kp_p * es; a.kp_h = p.kp_h * es; a.vp_p = p.vp_p * es; a.vp_h = p.vp_h * es;
   a.ks_b = (int)p.kp_s * es; a.vs_b = (int)p.vp_s * es; a.row_b = p.D * es; a.D = p.D;
