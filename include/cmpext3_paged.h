@@ -126,7 +126,10 @@ size_t cmpext3_paged_attn_workspace_size(int dtype, int B, int H, int H_kv, int 
  * its pages followed by -1.
  *
  *   workspace : 16-byte aligned, at least cmpext3_paged_select_workspace_size
- *               bytes (else CMPEXT3_E_INVALID); its contents do not matter.
+ *               bytes (else CMPEXT3_E_INVALID); its contents do not matter and
+ *               are overwritten (so it is not the attention's, whose counters
+ *               have to stay zero).  Calls that run one after another may share
+ *               it, from any thread.
  */
 int cmpext3_paged_select(const void* q, const void* key_bounds, int32_t* selected,
                          int dtype, int B, int H, int H_kv, int D, int num_pages, int page_size,

@@ -4,8 +4,18 @@
 #include <stdint.h>
 #include <string.h>
 
+#include <mutex>
+
 #include "../../include/cmpext3_paged.h"
 #include "paged_common.h"
+
+namespace cmpext3 {
+// Held while a call's launches are submitted to a workspace (attn_abi.cpp): a
+// selection hands its scores from one launch to the next there, and the
+// attention calls that share a stream's workspace hand over mask bits, so no
+// other call's launch may come between.
+std::mutex& space_lock(const void* space);
+}  // namespace cmpext3
 
 namespace {
 
@@ -172,6 +182,8 @@ int cmpext3_paged_attn(const void* q, const void* k_pages, const void* v_pages, 
   p.q_sign = scale < 0.f ? (es == 4 ? 0x80000000u : 0x80008000u) : 0u;
   p.workspace = workspace;
   p.workspace_bytes = workspace ? workspace_bytes : 0;
+  std::unique_lock<std::mutex> submit(cmpext3::space_lock(workspace), std::defer_lock);
+  if (p.workspace) submit.lock();
   return done(cmpext3::launch_paged_attn(p, dtype, stream));
 }
 
@@ -208,6 +220,8 @@ int cmpext3_paged_select(const void* q, const void* key_bounds, int32_t* selecte
   p.map = map_of(page_table, table_width, table_stride, seq_lens, nullptr, num_pages, page_size);
   p.n_selected = n_selected;
   p.workspace = workspace;
+  std::unique_lock<std::mutex> submit(cmpext3::space_lock(workspace), std::defer_lock);
+  if (workspace) submit.lock();
   return done(cmpext3::launch_paged_select(p, dtype, stream));
 }
 
