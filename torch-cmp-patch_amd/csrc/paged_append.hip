@@ -22,56 +22,70 @@ namespace cmpext3 {
 
 namespace {
 
-template <typename T> struct Elem;
-template <> struct Elem<_Float16> {
-  static constexpr int N = 8;  // elements of a 16-byte chunk
-  static __device__ float get(const u32x4& w, int e) {
-    return (float)__builtin_bit_cast(_Float16, (uint16_t)(w[e >> 1] >> (16 * (e & 1))));
-  }
-  static __device__ u32x4 put(const float* x) {
+template <typename T>
+__device__ __forceinline__ float get_elem(uint32_t w, int e) {
+  if constexpr (sizeof(T) == 4) return __uint_as_float(w);
+  else if constexpr (__is_same(T, __bf16)) return __uint_as_float(e & 1 ? w & 0xffff0000u : w << 16);
+  else return (float)__builtin_bit_cast(_Float16, (uint16_t)(w >> (16 * (e & 1))));
+}
+
+// The elements of a 16-byte chunk.
+template <typename T>
+struct Elem {
+  static constexpr int N = 16 / (int)sizeof(T);
+  static __device__ __forceinline__ float get(const u32x4& w, int e) { return get_elem<T>(w[e * (int)sizeof(T) / 4], e); }
+  static __device__ __forceinline__ u32x4 put(const float* x) {
     u32x4 w;
 #pragma unroll
-    for (int i = 0; i < 4; ++i)
-      w[i] = (uint32_t)__builtin_bit_cast(uint16_t, (_Float16)x[2 * i]) |
-             (uint32_t)__builtin_bit_cast(uint16_t, (_Float16)x[2 * i + 1]) << 16;
+    for (int i = 0; i < 4; ++i) {
+      if constexpr (sizeof(T) == 4)
+        w[i] = __float_as_uint(x[i]);
+      else
+        w[i] = (uint32_t)__builtin_bit_cast(uint16_t, (T)x[2 * i]) |
+               (uint32_t)__builtin_bit_cast(uint16_t, (T)x[2 * i + 1]) << 16;
+    }
     return w;
   }
-  static __device__ u32x4 nan() { return (u32x4){0x7fff7fffu, 0x7fff7fffu, 0x7fff7fffu, 0x7fff7fffu}; }
-};
-template <> struct Elem<__bf16> {
-  static constexpr int N = 8;
-  static __device__ float get(const u32x4& w, int e) {
-    return __uint_as_float(e & 1 ? w[e >> 1] & 0xffff0000u : w[e >> 1] << 16);
-  }
-  static __device__ u32x4 put(const float* x) {
+  static __device__ __forceinline__ u32x4 all(uint32_t v) {
     u32x4 w;
 #pragma unroll
-    for (int i = 0; i < 4; ++i)
-      w[i] = (uint32_t)__builtin_bit_cast(uint16_t, (__bf16)x[2 * i]) |
-             (uint32_t)__builtin_bit_cast(uint16_t, (__bf16)x[2 * i + 1]) << 16;
+    for (int i = 0; i < 4; ++i) w[i] = v;
     return w;
   }
-  static __device__ u32x4 nan() { return (u32x4){0x7fff7fffu, 0x7fff7fffu, 0x7fff7fffu, 0x7fff7fffu}; }
+  static __device__ __forceinline__ u32x4 nan() { return all(sizeof(T) == 4 ? 0x7fc00000u : 0x7fff7fffu); }
 };
-template <> struct Elem<float> {
-  static constexpr int N = 4;
-  static __device__ float get(const u32x4& w, int e) { return __uint_as_float(w[e]); }
-  static __device__ u32x4 put(const float* x) {
-    return (u32x4){__float_as_uint(x[0]), __float_as_uint(x[1]), __float_as_uint(x[2]), __float_as_uint(x[3])};
+
+// N angles' cosines or sines.
+template <int N>
+__device__ __forceinline__ void angles(const float* at, float* x) {
+  typedef f32x4 four __attribute__((aligned(4)));
+  typedef u32x2 two __attribute__((aligned(4)));
+  if constexpr (N % 4 == 0) {
+#pragma unroll
+    for (int k = 0; k < N; k += 4) {
+      const f32x4 v = *(const four*)(at + k);
+      x[k] = v[0]; x[k + 1] = v[1]; x[k + 2] = v[2]; x[k + 3] = v[3];
+    }
+  } else {
+    static_assert(N == 2, "a chunk's pairs");
+    const u32x2 v = *(const two*)at;
+    x[0] = __uint_as_float(v[0]);
+    x[1] = __uint_as_float(v[1]);
   }
-  static __device__ u32x4 nan() { return (u32x4){0x7fc00000u, 0x7fc00000u, 0x7fc00000u, 0x7fc00000u}; }
-};
+}
 
 // How a row is rotated.
 enum Mode {
   kCopy,   // not at all
-  kHalf,   // pairs (d, d + rot / 2) in whole chunks
+  kHalf,   // pairs (d, d + rot / 2) in whole 16-byte chunks
+  kSkew,   // the same where a half is no whole number of chunks
   kSide,   // pairs (2 d, 2 d + 1) in whole chunks
   kAny     // anything else: element by element
 };
 
 struct Shape {
-  int units, pairs;  // units of a row; the first `pairs` of them are two chunks, `pairs` apart
+  int units, pairs;  // units of a row; the first `pairs` of them are two chunks, a half apart
+  int half, rest;    // channels of a half, and behind the rotated ones
   int heads;         // heads of a token in the first section: V and Q, and K where it takes no runs
   int runs;          // second section: runs per (sequence, head)
   int waves;         // waves of a run, 1 or 4
@@ -80,65 +94,65 @@ struct Shape {
   Div by_units, by_heads, by_s, by_ps, by_runs, by_groups;
 };
 
-// One unit of a row: its chunks, and those rotated.
+// A chunk in memory: at a multiple of 16 bytes, or of 4.
+template <bool SKEW> struct Words { typedef u32x4 type; };
+template <> struct Words<true> { typedef u32x4 type __attribute__((aligned(4))); };
+
+// One unit of a row: a chunk or two, and those rotated.
 template <typename T, int MODE>
 struct Unit {
-  static constexpr int N = Elem<T>::N;
-  int c0, c1;  // c1 < 0: one chunk
+  typedef Elem<T> E;
+  static constexpr int N = E::N;
+  static constexpr bool kTwo = MODE == kHalf || MODE == kSkew;  // the chunks of a pair turn together
+  typedef typename Words<MODE == kSkew>::type W;
+  int e0, e1;  // the chunks' first channels; e1 < 0: one chunk
   u32x4 x0, x1;
   __device__ __forceinline__ Unit(int u, const Shape& sh) {
-    if constexpr (MODE == kHalf) {
-      c0 = u < sh.pairs ? u : u + sh.pairs;
-      c1 = u < sh.pairs ? u + sh.pairs : -1;
-    } else {
-      c0 = u;
-      c1 = -1;
+    e0 = kTwo && u >= sh.pairs ? u * N - sh.pairs * N : u * N;
+    if constexpr (MODE == kSkew) {
+      // the last chunk of a part ends with it: what it shares with the one
+      // before is written twice, the same
+      e0 = u < sh.pairs ? min(e0, sh.half - N) : 2 * sh.half + min(e0, sh.rest - N);
+    } else if (kTwo && u >= sh.pairs) {
+      e0 += 2 * sh.half;
     }
+    e1 = kTwo && u < sh.pairs ? e0 + sh.half : -1;
   }
   __device__ __forceinline__ void load(const T* row) {
-    x0 = *(const u32x4*)(row + c0 * N);
+    x0 = *(const W*)(row + e0);
     x1 = x0;
-    if constexpr (MODE == kHalf) {
-      if (c1 >= 0) x1 = *(const u32x4*)(row + c1 * N);
+    if constexpr (kTwo) {
+      if (e1 >= 0) x1 = *(const W*)(row + e1);
     }
   }
   // by the angles of one row of the tables
   __device__ __forceinline__ void rotate(const T* row, const AppendParams& p, const float* cs, const float* sn) {
-    const int d0 = c0 * N;
-    if constexpr (MODE == kHalf) {
-      if (c1 < 0) return;
-      float a[N], b[N];
-      f32x4 c[N / 4], s[N / 4];
-#pragma unroll
-      for (int k = 0; k < N / 4; ++k) {
-        c[k] = *(const f32x4*)(cs + d0 + 4 * k);
-        s[k] = *(const f32x4*)(sn + d0 + 4 * k);
-      }
+    const int d0 = e0;
+    if constexpr (kTwo) {
+      if (e1 < 0) return;
+      float a[N], b[N], c[N], s[N];
+      angles<N>(cs + d0, c);
+      angles<N>(sn + d0, s);
 #pragma unroll
       for (int e = 0; e < N; ++e) {
-        const float x = Elem<T>::get(x0, e), y = Elem<T>::get(x1, e), cc = c[e / 4][e % 4], ss = s[e / 4][e % 4];
-        a[e] = x * cc - y * ss;
-        b[e] = y * cc + x * ss;
+        const float x = E::get(x0, e), y = E::get(x1, e);
+        a[e] = x * c[e] - y * s[e];
+        b[e] = y * c[e] + x * s[e];
       }
-      x0 = Elem<T>::put(a);
-      x1 = Elem<T>::put(b);
+      x0 = E::put(a);
+      x1 = E::put(b);
     } else if constexpr (MODE == kSide) {
       if (d0 >= p.rot) return;
       float a[N], c[N / 2], s[N / 2];
-      if constexpr (N == 8) {
-        *(f32x4*)c = *(const f32x4*)(cs + d0 / 2);
-        *(f32x4*)s = *(const f32x4*)(sn + d0 / 2);
-      } else {
-        *(u32x2*)c = *(const u32x2*)(cs + d0 / 2);
-        *(u32x2*)s = *(const u32x2*)(sn + d0 / 2);
-      }
+      angles<N / 2>(cs + d0 / 2, c);
+      angles<N / 2>(sn + d0 / 2, s);
 #pragma unroll
       for (int e = 0; e < N; e += 2) {
-        const float x = Elem<T>::get(x0, e), y = Elem<T>::get(x0, e + 1);
+        const float x = E::get(x0, e), y = E::get(x0, e + 1);
         a[e] = x * c[e / 2] - y * s[e / 2];
         a[e + 1] = y * c[e / 2] + x * s[e / 2];
       }
-      x0 = Elem<T>::put(a);
+      x0 = E::put(a);
     } else if constexpr (MODE == kAny) {
       const int h = p.rot / 2;
       if (d0 >= p.rot) return;
@@ -148,29 +162,31 @@ struct Unit {
         const int d = d0 + e;
         const int j = p.interleaved ? d / 2 : d < h ? d : d - h;
         const bool low = p.interleaved ? (d & 1) == 0 : d < h;
-        const float x = Elem<T>::get(x0, e);
+        const float x = E::get(x0, e);
         a[e] = x;
         if (d < p.rot) {
           const float y = (float)row[p.interleaved ? (low ? d + 1 : d - 1) : (low ? d + h : d - h)];
           a[e] = low ? x * cs[j] - y * sn[j] : x * cs[j] + y * sn[j];
         }
       }
-      x0 = Elem<T>::put(a);
+      x0 = E::put(a);
     }
   }
   __device__ __forceinline__ void store(T* row) const {
-    *(u32x4*)(row + c0 * N) = x0;
-    if constexpr (MODE == kHalf) {
-      if (c1 >= 0) *(u32x4*)(row + c1 * N) = x1;
+    *(W*)(row + e0) = x0;
+    if constexpr (kTwo) {
+      if (e1 >= 0) *(W*)(row + e1) = x1;
     }
   }
   __device__ __forceinline__ void fill(const u32x4& w) { x0 = x1 = w; }
 };
 
 // Lowest and highest values of one chunk's channels.
-template <typename T>
+template <typename U>
 struct Range {
-  static constexpr int N = Elem<T>::N;
+  typedef typename U::E E;
+  typedef typename U::W W;
+  static constexpr int N = E::N;
   float lo[N], hi[N];
   __device__ __forceinline__ void clear() {
 #pragma unroll
@@ -182,8 +198,8 @@ struct Range {
   __device__ __forceinline__ void take(const u32x4& w) {
 #pragma unroll
     for (int e = 0; e < N; ++e) {
-      lo[e] = fminf(lo[e], Elem<T>::get(w, e));
-      hi[e] = fmaxf(hi[e], Elem<T>::get(w, e));
+      lo[e] = fminf(lo[e], E::get(w, e));
+      hi[e] = fmaxf(hi[e], E::get(w, e));
     }
   }
   __device__ __forceinline__ void take(const Range& o) {
@@ -205,24 +221,25 @@ struct Range {
       }
     }
   }
+  template <typename T>
   __device__ __forceinline__ void store(T* lows, T* highs, bool anew) {
     if (!anew) {
-      const u32x4 a = *(const u32x4*)lows, z = *(const u32x4*)highs;
+      const u32x4 a = *(const W*)lows, z = *(const W*)highs;
 #pragma unroll
       for (int e = 0; e < N; ++e) {
-        lo[e] = fminf(lo[e], Elem<T>::get(a, e));
-        hi[e] = fmaxf(hi[e], Elem<T>::get(z, e));
+        lo[e] = fminf(lo[e], E::get(a, e));
+        hi[e] = fmaxf(hi[e], E::get(z, e));
       }
     }
-    *(u32x4*)lows = Elem<T>::put(lo);
-    *(u32x4*)highs = Elem<T>::put(hi);
+    *(W*)lows = E::put(lo);
+    *(W*)highs = E::put(hi);
   }
 };
 
 // Keys of a run with their page's bounds.
 template <typename T, int MODE>
 __device__ __forceinline__ void append_run(const AppendParams& p, const Shape& sh, int wg) {
-  constexpr int N = Elem<T>::N;
+  typedef Unit<T, MODE> U;
   const int lane = thread_x() & 63, wave = __builtin_amdgcn_readfirstlane(thread_x() >> 6);
   const int rest = quot(wg, sh.by_runs.m, sh.by_runs.s), run = wg - rest * sh.runs;
   const int heads = 4 / sh.waves, groups = (p.Hkv + heads - 1) / heads;  // a workgroup's heads
@@ -241,7 +258,7 @@ __device__ __forceinline__ void append_run(const AppendParams& p, const Shape& s
   const T* src = (const T*)p.k + b * p.k_b + head * p.k_h;
   T* dst = (T*)p.k_pages + page * p.kp_p + head * p.kp_h;
   const Unit<T, MODE> at(u, sh);
-  Range<T> r0, r1;
+  Range<U> r0, r1;
   r0.clear();
   r1.clear();
   bool some = false;
@@ -260,44 +277,44 @@ __device__ __forceinline__ void append_run(const AppendParams& p, const Shape& s
       if (ok) {
         w.store(dst + (i - start) * p.kp_s);
         r0.take(w.x0);
-        if constexpr (MODE == kHalf) r1.take(w.x1);
+        if constexpr (Unit<T, MODE>::kTwo) r1.take(w.x1);
         some = true;
       }
     }
   }
   if (sh.waves == 1 && !__builtin_amdgcn_ballot_w64(some)) return;
   r0.join(lane, t, TL, sh.units);
-  if constexpr (MODE == kHalf) r1.join(lane, t, TL, sh.units);
+  if constexpr (Unit<T, MODE>::kTwo) r1.join(lane, t, TL, sh.units);
   if (sh.waves > 1) {  // the four waves' bounds meet in the first
-    __shared__ Range<T> far[3][2][64];
+    __shared__ Range<U> far[3][2][64];
     __shared__ int any;
     if (thread_x() == 0) any = 0;
     __syncthreads();
     if (some) any = 1;
     if (wave > 0 && t == 0) {
       far[wave - 1][0][lane] = r0;
-      if constexpr (MODE == kHalf) far[wave - 1][1][lane] = r1;
+      if constexpr (Unit<T, MODE>::kTwo) far[wave - 1][1][lane] = r1;
     }
     __syncthreads();
     if (wave > 0 || !any) return;
     if (t == 0)
       for (int w = 0; w < 3; ++w) {
         r0.take(far[w][0][lane]);
-        if constexpr (MODE == kHalf) r1.take(far[w][1][lane]);
+        if constexpr (Unit<T, MODE>::kTwo) r1.take(far[w][1][lane]);
       }
   }
   if (t != 0) return;
   const bool anew = start >= 0;  // the page begins with a new token
   T* edge = (T*)p.bounds + page * p.kb_p + head * p.kb_h;
-  r0.store(edge + at.c0 * N, edge + p.kb_e + at.c0 * N, anew);
-  if constexpr (MODE == kHalf) {
-    if (at.c1 >= 0) r1.store(edge + at.c1 * N, edge + p.kb_e + at.c1 * N, anew);
+  r0.store(edge + at.e0, edge + p.kb_e + at.e0, anew);
+  if constexpr (Unit<T, MODE>::kTwo) {
+    if (at.e1 >= 0) r1.store(edge + at.e1, edge + p.kb_e + at.e1, anew);
   }
 }
 
 template <typename T, int MODE>
 __global__ __launch_bounds__(256) void paged_append(AppendParams p, Shape sh) {
-  constexpr int N = Elem<T>::N;
+  typedef Unit<T, MODE> U;
   if (block_x() >= sh.first) {
     append_run<T, MODE>(p, sh, block_x() - sh.first);
     return;
@@ -328,8 +345,8 @@ __global__ __launch_bounds__(256) void paged_append(AppendParams p, Shape sh) {
     if (kind != 1 && ok) w.rotate(row, p, p.cos + a * p.rot_s, p.sin + a * p.rot_s);
   }
   if (kind == 2) {
-    if (!fresh) w.fill((u32x4){0u, 0u, 0u, 0u});
-    else if (!ok) w.fill(Elem<T>::nan());
+    if (!fresh) w.fill(U::E::all(0));
+    else if (!ok) w.fill(U::E::nan());
     w.store((T*)p.q_out + b * p.o_b + head * p.o_h + i * p.o_s);
     return;
   }
@@ -338,16 +355,16 @@ __global__ __launch_bounds__(256) void paged_append(AppendParams p, Shape sh) {
                     : (T*)p.v_pages + page * p.vp_p + head * p.vp_h + slot * p.vp_s);
   if (kind == 0 && p.bounds) {  // one token a call: its page's bounds are this unit's alone
     T* edge = (T*)p.bounds + page * p.kb_p + head * p.kb_h;
-    Range<T> r;
+    Range<U> r;
     r.clear();
     r.take(w.x0);
-    r.store(edge + w.c0 * N, edge + p.kb_e + w.c0 * N, slot == 0);
-    if constexpr (MODE == kHalf) {
-      if (w.c1 >= 0) {
-        Range<T> z;
+    r.store(edge + w.e0, edge + p.kb_e + w.e0, slot == 0);
+    if constexpr (Unit<T, MODE>::kTwo) {
+      if (w.e1 >= 0) {
+        Range<U> z;
         z.clear();
         z.take(w.x1);
-        z.store(edge + w.c1 * N, edge + p.kb_e + w.c1 * N, slot == 0);
+        z.store(edge + w.e1, edge + p.kb_e + w.e1, slot == 0);
       }
     }
   }
@@ -355,20 +372,24 @@ __global__ __launch_bounds__(256) void paged_append(AppendParams p, Shape sh) {
 
 template <typename T>
 hipError_t launch(const AppendParams& p, hipStream_t s) {
-  constexpr int N = Elem<T>::N;
-  // chunks turn whole where halves, or the rotated part, are whole chunks and
-  // the tables' rows are read in 16 bytes
-  const int h = p.rot / 2;
-  const bool tables = (((uintptr_t)p.cos | (uintptr_t)p.sin) & 15u) == 0 && p.rot_s % 4 == 0;
-  const Mode mode = p.rot == 0                                               ? kCopy
-                    : tables && !p.interleaved && h % N == 0                ? kHalf
-                    : tables && p.interleaved && p.rot % N == 0             ? kSide
-                                                                            : kAny;
-  Shape sh;
-  const int chunks = p.D / N, ps = p.map.page_size;
-  sh.pairs = mode == kHalf ? h / N : 0;
-  sh.units = chunks - sh.pairs;
+  constexpr int N = 16 / (int)sizeof(T);
+  const int h = p.rot / 2, ps = p.map.page_size;
   const bool by_runs = p.bounds && p.S > 1;
+  Shape sh;
+  sh.half = h;
+  sh.rest = p.D - p.rot;
+  // halves that are no whole chunks take skewed ones, where each part of the
+  // row holds one and words keep their 4 bytes (bf16 [36,20/5,1081,72] with 36
+  // rotated: 92.7 us, element by element 136)
+  const bool skew = h >= N && h * sizeof(T) % 4 == 0 && (sh.rest == 0 || sh.rest >= N);
+  const Mode mode = p.rot == 0        ? kCopy
+                    : p.interleaved   ? (p.rot % N == 0 ? kSide : kAny)
+                    : h % N == 0      ? kHalf
+                    : skew            ? kSkew
+                                      : kAny;
+  const bool two = mode == kHalf || mode == kSkew;
+  sh.pairs = two ? (h + N - 1) / N : 0;
+  sh.units = two ? sh.pairs + (sh.rest + N - 1) / N : p.D / N;
   sh.v_at = by_runs ? 0 : p.Hkv;
   sh.q_at = sh.v_at + p.Hkv;
   sh.heads = sh.q_at + p.H;
@@ -389,6 +410,7 @@ hipError_t launch(const AppendParams& p, hipStream_t s) {
   const dim3 grid((unsigned)(sh.first + second)), block(256);
   if (mode == kCopy) hipLaunchKernelGGL((paged_append<T, kCopy>), grid, block, 0, s, p, sh);
   else if (mode == kHalf) hipLaunchKernelGGL((paged_append<T, kHalf>), grid, block, 0, s, p, sh);
+  else if (mode == kSkew) hipLaunchKernelGGL((paged_append<T, kSkew>), grid, block, 0, s, p, sh);
   else if (mode == kSide) hipLaunchKernelGGL((paged_append<T, kSide>), grid, block, 0, s, p, sh);
   else hipLaunchKernelGGL((paged_append<T, kAny>), grid, block, 0, s, p, sh);
   return hipGetLastError();

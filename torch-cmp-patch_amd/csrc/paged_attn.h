@@ -77,7 +77,7 @@ template <> struct Mma<__bf16> {
 constexpr int kRows = 16;        // query rows of a block
 constexpr int kTile = 16;        // slots of a tile
 constexpr int kMaxWgs = 1024;    // workgroups of a launch at most (counters: one each)
-constexpr int kMinTiles = 16;    // tiles of a workgroup's share at least
+constexpr int kF32Min = 2;
 constexpr int kSetup = 6;        // what a unit costs beside its tiles, in tiles
 constexpr int kShortCut = 40;    // tiles of a part up to which units are cut by themselves
 constexpr int kLongShare = 48;   // tiles of a share from which one workgroup a CU is enough
@@ -98,6 +98,10 @@ constexpr int pg_lds(int dk, int es) {
   const int states = nw * kRows * (dk + 6) * 4;
   return ring > states ? ring : states;
 }
+
+// Tiles of a workgroup's share at least: four a wave (two in fp32, whose products
+// take longer).
+constexpr int pg_min_tiles(int dk, int es) { return pg_waves(dk * es) * (es == 4 ? kF32Min : 4); }
 
 // Blocks of 16 query rows that a unit takes together, each K and V fragment read
 // once for all of them: as many as the rows fill and half of the registers hold
@@ -216,6 +220,7 @@ __global__ __launch_bounds__(pg_waves(DK * sizeof(T)) * 64, pg_waves(DK * sizeof
   // products take longer).  bf16 [1,16/8,1,300,128] 7.7 us whole, 10.7 in parts;
   // fp32 [2,20/5,2,500,128] 18.7 us with 32 here, 12.2 with 16.
   constexpr int kWhole = F32 ? 16 : 32;
+  constexpr int kMinTiles = pg_min_tiles(DK, ES);
   constexpr int RING = NW * NS * STAGE;
   static_assert(BLK % 1024 == 0 && NC % 4 == 0 && (!F32 || DK % 64 == 0), "head dim bucket");
   static_assert(NS >= 1 && IPT * (NS - 1) <= 63, "vmcnt range");
@@ -278,7 +283,9 @@ __global__ __launch_bounds__(pg_waves(DK * sizeof(T)) * 64, pg_waves(DK * sizeof
   int cut = 0;          // > 0: units are cut by themselves
   auto weight_of = [](int tiles) { return tiles > 0 ? tiles + kSetup : 0; };
   auto parts_of = [&](int tiles, int cut) {
-    return tiles == 0 ? 0 : tiles <= kWhole ? 1 : (int)((uint32_t)(weight_of(tiles) + cut - 1) / (uint32_t)cut);
+    if (tiles <= kWhole) return tiles == 0 ? 0 : 1;
+    const int n = (int)((uint32_t)(weight_of(tiles) + cut - 1) / (uint32_t)cut);
+    return n > kJoin && n <= kJoin + kJoin / 2 ? kJoin : n;  // a little longer sweeps for a level of the join
   };
   // sequence i of the batch, the same for every lane
   auto seq_at = [&](int i) {

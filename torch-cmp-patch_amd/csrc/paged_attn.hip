@@ -44,7 +44,7 @@ int workgroups(int dtype, int B, int H, int Hkv, int S, int D, int page_size, in
   const int64_t units = unit_count(dtype, B, H, Hkv, S, D);
   const int64_t cols = n_selected > 0 ? n_selected : width;
   const int64_t tiles = units * cols * ((page_size + kTile - 1) / kTile);
-  const int64_t most = units + (tiles + kSetup * units) / kMinTiles;
+  const int64_t most = units + (tiles + kSetup * units) / pg_min_tiles(bucket(dtype, D), dtype == 2 ? 4 : 2);
   return most < n ? (int)most : n;
 }
 
