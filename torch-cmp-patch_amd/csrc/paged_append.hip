@@ -88,7 +88,6 @@ struct Shape {
   int half, rest;    // channels of a half, and behind the rotated ones
   int heads;         // heads of a token in the first section: V and Q, and K where it takes no runs
   int runs;          // second section: runs per (sequence, head)
-  int waves;         // waves of a run, 1 or 4
   int first;         // workgroups of the first section
   int q_at, v_at;    // where V's and Q's heads begin in a token's
   Div by_units, by_heads, by_s, by_ps, by_runs, by_groups;
@@ -237,14 +236,15 @@ struct Range {
 };
 
 // Keys of a run with their page's bounds.
-template <typename T, int MODE>
+template <typename T, int MODE, int WAVES>
 __device__ __forceinline__ void append_run(const AppendParams& p, const Shape& sh, int wg) {
   typedef Unit<T, MODE> U;
   const int lane = thread_x() & 63, wave = __builtin_amdgcn_readfirstlane(thread_x() >> 6);
   const int rest = quot(wg, sh.by_runs.m, sh.by_runs.s), run = wg - rest * sh.runs;
-  const int heads = 4 / sh.waves, groups = (p.Hkv + heads - 1) / heads;  // a workgroup's heads
+  constexpr int heads = 4 / WAVES;  // a workgroup's
+  const int groups = (p.Hkv + heads - 1) / heads;
   const int b = quot(rest, sh.by_groups.m, sh.by_groups.s);
-  const int head = (rest - b * groups) * heads + (sh.waves == 1 ? wave : 0);
+  const int head = (rest - b * groups) * heads + (WAVES == 1 ? wave : 0);
   if (head >= p.Hkv) return;
   const int len = seq_len(p.map, b), n = seq_new(p.map, b, p.S, len);
   const int pos0 = len - n, ps = p.map.page_size;
@@ -264,7 +264,7 @@ __device__ __forceinline__ void append_run(const AppendParams& p, const Shape& s
   bool some = false;
   if (t < TL) {
 #pragma unroll 2
-    for (int i = i0 + t + (sh.waves == 1 ? 0 : wave * TL); i < i1; i += TL * sh.waves) {
+    for (int i = i0 + t + (WAVES == 1 ? 0 : wave * TL); i < i1; i += TL * WAVES) {
       const T* row = src + i * p.k_s;
       Unit<T, MODE> w = at;
       w.load(row);
@@ -282,10 +282,10 @@ __device__ __forceinline__ void append_run(const AppendParams& p, const Shape& s
       }
     }
   }
-  if (sh.waves == 1 && !__builtin_amdgcn_ballot_w64(some)) return;
+  if (WAVES == 1 && !__builtin_amdgcn_ballot_w64(some)) return;
   r0.join(lane, t, TL, sh.units);
   if constexpr (Unit<T, MODE>::kTwo) r1.join(lane, t, TL, sh.units);
-  if (sh.waves > 1) {  // the four waves' bounds meet in the first
+  if constexpr (WAVES > 1) {  // the four waves' bounds meet in the first
     __shared__ Range<U> far[3][2][64];
     __shared__ int any;
     if (thread_x() == 0) any = 0;
@@ -312,12 +312,17 @@ __device__ __forceinline__ void append_run(const AppendParams& p, const Shape& s
   }
 }
 
-template <typename T, int MODE>
+// RUNS: waves of a run in the second section, 0 without one (its registers, and
+// the LDS of four waves, would cost the others residency: fp16 chunks 10.1 us
+// with it compiled in, 9.5 without).
+template <typename T, int MODE, int RUNS>
 __global__ __launch_bounds__(256) void paged_append(AppendParams p, Shape sh) {
   typedef Unit<T, MODE> U;
-  if (block_x() >= sh.first) {
-    append_run<T, MODE>(p, sh, block_x() - sh.first);
-    return;
+  if constexpr (RUNS > 0) {
+    if (block_x() >= sh.first) {
+      append_run<T, MODE, RUNS>(p, sh, block_x() - sh.first);
+      return;
+    }
   }
   const int item = block_x() * 256 + thread_x();
   const int rest = quot(item, sh.by_units.m, sh.by_units.s), u = item - rest * sh.units;
@@ -370,6 +375,16 @@ __global__ __launch_bounds__(256) void paged_append(AppendParams p, Shape sh) {
   }
 }
 
+template <typename T, int RUNS>
+void launch_mode(const AppendParams& p, const Shape& sh, Mode mode, unsigned wgs, hipStream_t s) {
+  const dim3 grid(wgs), block(256);
+  if (mode == kCopy) hipLaunchKernelGGL((paged_append<T, kCopy, RUNS>), grid, block, 0, s, p, sh);
+  else if (mode == kHalf) hipLaunchKernelGGL((paged_append<T, kHalf, RUNS>), grid, block, 0, s, p, sh);
+  else if (mode == kSkew) hipLaunchKernelGGL((paged_append<T, kSkew, RUNS>), grid, block, 0, s, p, sh);
+  else if (mode == kSide) hipLaunchKernelGGL((paged_append<T, kSide, RUNS>), grid, block, 0, s, p, sh);
+  else hipLaunchKernelGGL((paged_append<T, kAny, RUNS>), grid, block, 0, s, p, sh);
+}
+
 template <typename T>
 hipError_t launch(const AppendParams& p, hipStream_t s) {
   constexpr int N = 16 / (int)sizeof(T);
@@ -380,7 +395,7 @@ hipError_t launch(const AppendParams& p, hipStream_t s) {
   sh.rest = p.D - p.rot;
   // halves that are no whole chunks take skewed ones, where each part of the
   // row holds one and words keep their 4 bytes (bf16 [36,20/5,1081,72] with 36
-  // rotated: 92.7 us, element by element 136)
+  // rotated: 77 us, element by element 136)
   const bool skew = h >= N && h * sizeof(T) % 4 == 0 && (sh.rest == 0 || sh.rest >= N);
   const Mode mode = p.rot == 0        ? kCopy
                     : p.interleaved   ? (p.rot % N == 0 ? kSide : kAny)
@@ -398,8 +413,8 @@ hipError_t launch(const AppendParams& p, hipStream_t s) {
   // pages that S tokens beginning in any slot touch at most
   sh.runs = by_runs ? (p.S - 1 + ps - 1) / ps + 1 : 1;
   // a run of more tokens than a wave takes in two steps goes to four waves
-  sh.waves = by_runs && (ps < p.S ? ps : p.S) * sh.units > 2 * 64 ? 4 : 1;
-  const int heads = 4 / sh.waves, groups = (p.Hkv + heads - 1) / heads;
+  const int waves = by_runs && (ps < p.S ? ps : p.S) * sh.units > 2 * 64 ? 4 : 1;
+  const int heads = 4 / waves, groups = (p.Hkv + heads - 1) / heads;
   const int64_t second = by_runs ? (int64_t)p.B * groups * sh.runs : 0;
   sh.by_units = div_by(sh.units);
   sh.by_heads = div_by(sh.heads);
@@ -407,12 +422,10 @@ hipError_t launch(const AppendParams& p, hipStream_t s) {
   sh.by_ps = div_by(ps);
   sh.by_runs = div_by(sh.runs);
   sh.by_groups = div_by(groups);
-  const dim3 grid((unsigned)(sh.first + second)), block(256);
-  if (mode == kCopy) hipLaunchKernelGGL((paged_append<T, kCopy>), grid, block, 0, s, p, sh);
-  else if (mode == kHalf) hipLaunchKernelGGL((paged_append<T, kHalf>), grid, block, 0, s, p, sh);
-  else if (mode == kSkew) hipLaunchKernelGGL((paged_append<T, kSkew>), grid, block, 0, s, p, sh);
-  else if (mode == kSide) hipLaunchKernelGGL((paged_append<T, kSide>), grid, block, 0, s, p, sh);
-  else hipLaunchKernelGGL((paged_append<T, kAny>), grid, block, 0, s, p, sh);
+  const unsigned wgs = (unsigned)(sh.first + second);
+  if (!by_runs) launch_mode<T, 0>(p, sh, mode, wgs, s);
+  else if (waves == 1) launch_mode<T, 1>(p, sh, mode, wgs, s);
+  else launch_mode<T, 4>(p, sh, mode, wgs, s);
   return hipGetLastError();
 }
 
