@@ -1,5 +1,6 @@
 // C ABI of the paged key-value cache: argument checks and kernel dispatch.
 // Unsupported input is reported by return code and nothing is launched.
+#include <float.h>
 #include <math.h>
 #include <stdint.h>
 #include <string.h>
@@ -178,7 +179,9 @@ int cmpext3_paged_attn(const void* q, const void* k_pages, const void* v_pages, 
   p.map = map_of(page_table, table_width, table_stride, seq_lens, new_lens, num_pages, page_size);
   p.selected = selected;
   p.n_selected = selected ? n_selected : 0;
-  p.c = fabsf(scale) * cmpext3::kLog2e;
+  // above 0, so that a key left out stays at -inf: at the least normal number a
+  // finite score is 0 to every digit
+  p.c = fmaxf(fabsf(scale) * cmpext3::kLog2e, FLT_MIN);
   p.q_sign = scale < 0.f ? (es == 4 ? 0x80000000u : 0x80008000u) : 0u;
   p.workspace = workspace;
   p.workspace_bytes = workspace ? workspace_bytes : 0;

@@ -21,7 +21,8 @@
 //    load of the table per 64 tiles, checked there), read back by v_readlane.
 //  * Scores S^T = K Q^T and O^T = V^T P^T on 16x16 MFMAs (16x16x32 and 16x16x16
 //    for fp16 and bf16, 16x16x4 for fp32), exact online softmax in the exp2
-//    domain with fp32 state.  For fp16 and bf16 a weight enters the second
+//    domain with fp32 state (scaled and set off against the maximum in one fma,
+//    so that only the rounding of the common maximum stays, and cancels).  For fp16 and bf16 a weight enters the second
 //    product in two parts, its value rounded to the tensors' type and the
 //    rounded rest (the matrix units are idle for most of the time anyway), whose
 //    product with an infinity is no number: then the wave sweeps once more.
@@ -557,9 +558,11 @@ __global__ __launch_bounds__(pg_waves(DK * sizeof(T)) * 64, pg_waves(DK * sizeof
           slots_q[q] = slots_q[q + 1];
         }
 
-        f32x4 s[NR];
+        // fp32: four sums of every fourth product (shorter chains: sums closer to the
+        // exact ones, and no product waits for the last)
+        f32x4 s[NR], more[NR][3];
 #pragma unroll
-        for (int z = 0; z < NR; ++z) s[z] = (f32x4){0.f, 0.f, 0.f, 0.f};
+        for (int z = 0; z < NR; ++z) s[z] = more[z][0] = more[z][1] = more[z][2] = (f32x4){0.f, 0.f, 0.f, 0.f};
 #pragma unroll
         for (int ks = 0; ks < KS; ++ks) {
           const u32x4 kk = *(const u32x4*)(st + kro[ks]);
@@ -567,8 +570,10 @@ __global__ __launch_bounds__(pg_waves(DK * sizeof(T)) * 64, pg_waves(DK * sizeof
           for (int z = 0; z < NR; ++z) {
             if constexpr (F32) {
 #pragma unroll
-              for (int e = 0; e < 4; ++e)
-                s[z] = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(kk[e]), __uint_as_float(qf[z][ks][e]), s[z], 0, 0, 0);
+              for (int e = 0; e < 4; ++e) {
+                f32x4& sum = e == 0 ? s[z] : more[z][e - 1];
+                sum = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(kk[e]), __uint_as_float(qf[z][ks][e]), sum, 0, 0, 0);
+              }
             } else {
               s[z] = Mma<T>::qk(kk, qf[z][ks], s[z]);
             }
@@ -578,15 +583,16 @@ __global__ __launch_bounds__(pg_waves(DK * sizeof(T)) * 64, pg_waves(DK * sizeof
         u32x2 pb[NR], pl[NR];  // fp16, bf16: rounded weights, and what the rounding left
 #pragma unroll
         for (int z = 0; z < NR; ++z) {
+          if constexpr (F32) s[z] = (s[z] + more[z][0]) + (more[z][1] + more[z][2]);
           float xs[4];
 #pragma unroll
-          for (int e = 0; e < 4; ++e) xs[e] = s[z][e] * cmul;
+          for (int e = 0; e < 4; ++e) xs[e] = s[z][e];
           if (slots < kTile || pos + kTile > sure) {
 #pragma unroll
             for (int e = 0; e < 4; ++e)
               if (4 * g + e >= slots || pos + 4 * g + e >= limit[z]) xs[e] = -INFINITY;
           }
-          const float mt = rows_max(fmaxf(fmaxf(xs[0], xs[1]), fmaxf(xs[2], xs[3])));
+          const float mt = cmul * rows_max(fmaxf(fmaxf(xs[0], xs[1]), fmaxf(xs[2], xs[3])));
           if (__builtin_amdgcn_ballot_w64(mt > m_run[z])) {  // some row's maximum rises
             const float m_new = fmaxf(m_run[z], mt);
             const float alpha = weight(m_run[z], m_new);
@@ -597,7 +603,7 @@ __global__ __launch_bounds__(pg_waves(DK * sizeof(T)) * 64, pg_waves(DK * sizeof
           }
           const float m_sub = m_run[z] == -INFINITY ? 0.f : m_run[z];
 #pragma unroll
-          for (int e = 0; e < 4; ++e) pe[z][e] = fast_exp2(xs[e] - m_sub);
+          for (int e = 0; e < 4; ++e) pe[z][e] = fast_exp2(__builtin_fmaf(xs[e], cmul, -m_sub));
           l_run[z] += (pe[z][0] + pe[z][1]) + (pe[z][2] + pe[z][3]);
           if constexpr (!F32) {
             pb[z][0] = Mma<T>::pack(pe[z][0], pe[z][1]);
