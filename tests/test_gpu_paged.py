@@ -441,6 +441,50 @@ def test_captured_steps_replay_beside_eager_ones():
                 assert torch.equal(a, b)
 
 
+def test_a_captured_step_follows_growing_sequences():
+    """One graph of a decode step, replayed as sequences grow past pages and tiles, one ends and another begins: the
+    work is dealt out on the device, so every replay is the eager step of its lengths."""
+    c = Cache("bf16", [500, 15, 0, 300], 2, 128, 16, width=40)
+    c.table.copy_(torch.randperm(200, generator=c.g)[:160].reshape(4, 40).to(torch.int32))
+    P = 200
+    pools = [[torch.zeros(P, 2, 16, 128, dtype=torch.bfloat16, device="cuda") for _ in range(2)] for _ in range(2)]
+    bounds = [torch.zeros(P, 2, 2, 128, dtype=torch.bfloat16, device="cuda") for _ in range(2)]
+    cos, sin = tables(640, 128)
+    lens = c.lens.clone()
+    k, v, q = (torch.zeros(4, h, 1, 128, dtype=torch.bfloat16, device="cuda") for h in (2, 2, 8))
+
+    def step(pool, kb):
+        r = cmpext3.paged_append(k, v, *pool, c.table, lens, query=q, cos=cos, sin=sin, key_bounds=kb)
+        sel = cmpext3.paged_select(r, kb, c.table, lens, 16, 6)
+        return (r, sel, cmpext3.paged_attention(r, *pool, c.table, lens),
+                cmpext3.paged_attention(r, *pool, c.table, lens, selected=sel))
+
+    step(pools[0], bounds[0])
+    torch.cuda.synchronize()
+    for pool in pools:  # the keys that are there at the start
+        for t, seed in zip(pool, (1, 2)):
+            t.copy_(torch.randn(t.shape, generator=torch.Generator().manual_seed(seed)))
+    for kb in bounds:
+        kb.copy_(torch.stack([pools[0][0].amin(2), pools[0][0].amax(2)], 2))
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = step(pools[0], bounds[0])
+    for i in range(24):
+        if i == 7:
+            lens[0], lens[2] = 0, 0  # one ends ...
+        if i == 9:
+            lens[2] = 63             # ... another begins
+        lens.copy_(torch.where(lens > 0, lens + 1, lens))
+        for t in (k, v, q):
+            t.copy_(torch.randn(t.shape, generator=c.g))
+        graph.replay()
+        want = step(pools[1], bounds[1])
+        torch.cuda.synchronize()
+        for a, b in zip(out, want):
+            assert torch.equal(a, b), i
+        assert torch.equal(pools[0][0], pools[1][0]) and torch.equal(bounds[0], bounds[1])
+
+
 def test_streams_of_their_own():
     """Calls on two streams at once, each with its own workspace."""
     states = [_state(1), _state(2, (900, 2048, 4000))]

@@ -78,31 +78,32 @@ template <> struct Mma<__bf16> {
 constexpr int kRows = 16;        // query rows of a block
 constexpr int kTile = 16;        // slots of a tile
 constexpr int kMaxWgs = 1024;    // workgroups of a launch at most (counters: one each)
-constexpr int kF32Min = 2;
 constexpr int kSetup = 6;        // what a unit costs beside its tiles, in tiles
 constexpr int kShortCut = 40;    // tiles of a part up to which units are cut by themselves
 constexpr int kLongShare = 48;   // tiles of a share from which one workgroup a CU is enough
 constexpr int kJoin = 8;         // parts joined at once
 
-// Waves per workgroup and stages per wave: as many stages as 64 KB of LDS hold,
-// four at most, so that two workgroups fit a CU.  More in flight is no faster
-// (bf16 [16,16/8,4096,128]: 54.3 us with 128 KB a CU, 52.0 with 64).
-constexpr int kPerCu = 2;        // workgroups per CU at most
-constexpr int pg_waves(int rb) { return rb > 512 ? 2 : 4; }  // rb: bytes of a row in LDS
+// Waves per workgroup, workgroups per CU at most, and stages per wave: as many as
+// 64 KB of LDS hold, from one to four, so that two workgroups fit a CU (one where
+// a stage of fp32 above D = 128 takes more).  More in flight is no faster (bf16
+// [16,16/8,4096,128]: 54.3 us with 128 KB a CU, 52.0 with 64); two workgroups of
+// two waves are slower than one of four (fp32 [33,40/10,3,1000,192] 121.6 us, 88.5).
+constexpr int kWaves = 4;
+constexpr int kPerCu = 2;
 constexpr int pg_stages(int rb) {
-  const int n = 64 * 1024 / (pg_waves(rb) * 2 * kTile * rb);
+  const int n = 64 * 1024 / (kWaves * 2 * kTile * rb);
   return n < 1 ? 1 : n < 4 ? n : 4;
 }
 // LDS of a workgroup: the rings, later the waves' states in the same place
 constexpr int pg_lds(int dk, int es) {
-  const int nw = pg_waves(dk * es), ring = nw * pg_stages(dk * es) * 2 * kTile * dk * es;
+  const int nw = kWaves, ring = nw * pg_stages(dk * es) * 2 * kTile * dk * es;
   const int states = nw * kRows * (dk + 6) * 4;
   return ring > states ? ring : states;
 }
 
 // Tiles of a workgroup's share at least: four a wave (two in fp32, whose products
 // take longer).
-constexpr int pg_min_tiles(int dk, int es) { return pg_waves(dk * es) * (es == 4 ? kF32Min : 4); }
+constexpr int pg_min_tiles(int es) { return kWaves * (es == 4 ? 2 : 4); }
 
 // Blocks of 16 query rows that a unit takes together, each K and V fragment read
 // once for all of them: as many as the rows fill and half of the registers hold
@@ -141,7 +142,7 @@ struct AttnArgs {
   int B, S, U, cap;        // U: units of a sequence; cap: keys a table row holds
   int nsel, width, ps, tpp;  // tpp: tiles per page
   Div by_ps, by_tpp, by_blocks, by_s;
-  int split, exact, full;  // split 0: whole units, dealt out in turn; exact: pages are whole tiles; full: workgroups the CUs hold
+  int split, exact, full;  // split 0: whole units, dealt out in turn; exact: pages are whole tiles; full: workgroups the CUs hold, two each (0: one each)
   int G, blocks, rows, num_pages;  // query heads per K/V head, units and rows of a K/V head
   int slot_rows;                   // rows of a part in the workspace
   const char *k, *v;
@@ -202,11 +203,11 @@ __device__ __forceinline__ float rows_sum(float x) {
 }
 
 template <typename T, int DK, int NR, bool SEL>
-__global__ __launch_bounds__(pg_waves(DK * sizeof(T)) * 64, pg_waves(DK * sizeof(T)) / 2) void paged_attn(AttnArgs) {
+__global__ __launch_bounds__(kWaves * 64, pg_lds(DK, sizeof(T)) > 80 * 1024 ? 1 : 2) void paged_attn(AttnArgs) {
   constexpr bool F32 = sizeof(T) == 4;
   constexpr int ES = sizeof(T);
   constexpr int RB = DK * ES;           // bytes of a K/V row in LDS
-  constexpr int NW = pg_waves(RB), NS = pg_stages(RB), NT = NW * 64;
+  constexpr int NW = kWaves, NS = pg_stages(RB), NT = NW * 64;
   constexpr int NC = RB / 16;           // 16-byte chunks per row
   constexpr int BLK = kTile * RB;
   constexpr int IB = BLK / 1024;        // DMA instructions per 16 rows
@@ -221,7 +222,7 @@ __global__ __launch_bounds__(pg_waves(DK * sizeof(T)) * 64, pg_waves(DK * sizeof
   // products take longer).  bf16 [1,16/8,1,300,128] 7.7 us whole, 10.7 in parts;
   // fp32 [2,20/5,2,500,128] 18.7 us with 32 here, 12.2 with 16.
   constexpr int kWhole = F32 ? 16 : 32;
-  constexpr int kMinTiles = pg_min_tiles(DK, ES);
+  constexpr int kMinTiles = pg_min_tiles(ES);
   constexpr int RING = NW * NS * STAGE;
   static_assert(BLK % 1024 == 0 && NC % 4 == 0 && (!F32 || DK % 64 == 0), "head dim bucket");
   static_assert(NS >= 1 && IPT * (NS - 1) <= 63, "vmcnt range");
@@ -340,7 +341,7 @@ __global__ __launch_bounds__(pg_waves(DK * sizeof(T)) * 64, pg_waves(DK * sizeof
       if (cut > 0) {
         const int own = parts_of(held.tiles, cut), upto = wave_scan(own);
         const int last = __builtin_amdgcn_readlane(upto, 63) * U;
-        if (2 * last > p->full) depth = (NS + 1) / 2;
+        if (p->full > 0 && 2 * last > p->full) depth = (NS + 1) / 2;
         if (wg < last) {
           x = wg;
           hi = wg + 1;
@@ -883,7 +884,7 @@ __global__ __launch_bounds__(pg_waves(DK * sizeof(T)) * 64, pg_waves(DK * sizeof
 
 template <typename T, int DK, int NR>
 hipError_t launch_nr(const AttnArgs& a, int wgs, hipStream_t s) {
-  const dim3 grid(wgs), block(pg_waves(DK * sizeof(T)) * 64);
+  const dim3 grid(wgs), block(kWaves * 64);
   if (a.nsel > 0) hipLaunchKernelGGL((paged_attn<T, DK, NR, true>), grid, block, 0, s, a);
   else hipLaunchKernelGGL((paged_attn<T, DK, NR, false>), grid, block, 0, s, a);
   return hipGetLastError();

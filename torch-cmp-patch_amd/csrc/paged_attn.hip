@@ -44,7 +44,7 @@ int workgroups(int dtype, int B, int H, int Hkv, int S, int D, int page_size, in
   const int64_t units = unit_count(dtype, B, H, Hkv, S, D);
   const int64_t cols = n_selected > 0 ? n_selected : width;
   const int64_t tiles = units * cols * ((page_size + kTile - 1) / kTile);
-  const int64_t most = units + (tiles + kSetup * units) / pg_min_tiles(bucket(dtype, D), dtype == 2 ? 4 : 2);
+  const int64_t most = units + (tiles + kSetup * units) / pg_min_tiles(dtype == 2 ? 4 : 2);
   return most < n ? (int)most : n;
 }
 
@@ -73,7 +73,7 @@ hipError_t launch_paged_attn(const PagedAttnParams& p, int dtype, hipStream_t s)
   a.nsel = p.n_selected; a.width = p.map.width; a.ps = ps; a.tpp = tpp;
   a.by_ps = div_by(ps); a.by_tpp = div_by(tpp); a.by_blocks = div_by(blocks); a.by_s = div_by(p.S);
   a.exact = ps % kTile == 0;
-  a.full = full_house(dtype, p.D);
+  a.full = full_house(dtype, p.D) > device_cus() ? full_house(dtype, p.D) : 0;
   a.G = G; a.blocks = blocks; a.rows = G * p.S; a.slot_rows = slot_rows(dtype, p.D, G * p.S); a.num_pages = p.map.num_pages;
   a.k = (const char*)p.k; a.v = (const char*)p.v;
   a.kp_p = p.kp_p * es; a.kp_h = p.kp_h * es; a.vp_p = p.vp_p * es; a.vp_h = p.vp_h * es;
