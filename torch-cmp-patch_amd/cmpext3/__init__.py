@@ -35,6 +35,10 @@ kernels (``attention`` below, a torch.autograd.Function); everything else
 with live autograd still goes to stock.  Off by default, so the default
 behaviour is the reference's.
 
+Serving from a paged key-value cache (no counterpart in the reference):
+``paged_append``, ``paged_attention`` and ``paged_select`` below, functions of
+their own that no patch routes to.
+
 Only the attention op of the reference is in this package: its other patched
 ops (linear, conv, norms, activations, ...) and its NVML clock/power side
 effect are deliberately absent.

@@ -28,6 +28,8 @@
 // attention_fwd_lse / attention_bwd: the training pair (no reference
 // counterpart: the reference is forward-only, cmpext3/__init__.py:115-125),
 // used by cmpext3's autograd Function.
+//
+// The paged key-value cache's operators are in paged_binding.cpp.
 #include <algorithm>
 #include <cmath>
 #include <map>

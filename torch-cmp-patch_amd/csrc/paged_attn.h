@@ -2,35 +2,37 @@
 // K/V head, a long sweep over keys that lie in pages.
 //
 // Such a launch moves almost nothing but K and V and is bound by the bytes it
-// keeps in flight from HBM.  Nothing on the host knows the sequences' lengths,
-// so the work is dealt out on the device:
+// keeps in flight from HBM (measured on MI355X: bf16 [16,16/8,1,4096,128] 51.8
+// us, 5.2 TB/s; [1,16/8,1,131072,256] 189 us, 5.7 TB/s), small ones by the
+// latency of their dependent loads (bf16 [1,16/8,1,300,128] 8.4 us).  Nothing on
+// the host knows the sequences' lengths, so the work is dealt out on the device:
 //
 //  * A unit is a (sequence, K/V head, up to 64 query rows); its keys are cut
 //    into tiles of 16 slots, none across a page.  All units' tiles in a row are
 //    one sequence of work, of which every workgroup takes an equal, contiguous
-//    share (its prefix sum over the batch is the first thing a workgroup
-//    does), so ragged batches load the chip evenly and a single long sequence
-//    spreads over all of it.
+//    share (every wave sums over the batch first), so ragged batches load the
+//    chip evenly and a single long sequence spreads over all of it.  Short
+//    units stay whole; where shares are short, units are cut one by one.
 //  * A workgroup's share is a list of segments, each within one unit.  Its four
 //    waves take a segment's tiles in turn; every wave streams its own tiles
 //    through a ring of stages in LDS filled by buffer_load ... lds (no staging
 //    registers, no barriers), one buffer descriptor per tile: the page's
-//    address is in its base, 64 bits wide, and its last valid slot is its end,
+//    address is in its base, 48 bits wide, and its last valid slot is its end,
 //    so slots behind the sequence read as zeros whatever they hold.
-//  * A lane holds the page numbers of one of the wave's next 64 tiles (one
-//    load of the table per 64 tiles, checked there), read back by v_readlane.
+//  * A lane makes the descriptors of one of the wave's next 64 tiles (one load
+//    of the table per 64 tiles, checked there), read back by v_readlane.
 //  * Scores S^T = K Q^T and O^T = V^T P^T on 16x16 MFMAs (16x16x32 and 16x16x16
 //    for fp16 and bf16, 16x16x4 for fp32), exact online softmax in the exp2
 //    domain with fp32 state (scaled and set off against the maximum in one fma,
-//    so that only the rounding of the common maximum stays, and cancels).  For fp16 and bf16 a weight enters the second
-//    product in two parts, its value rounded to the tensors' type and the
-//    rounded rest (the matrix units are idle for most of the time anyway), whose
-//    product with an infinity is no number: then the wave sweeps once more.
+//    so that only the rounding of the common maximum stays, and cancels).  For
+//    fp16 and bf16 a weight enters the second product in two parts, its value
+//    rounded to the tensors' type and the rounded rest (the matrix units are
+//    idle for most of the time anyway), whose product with an infinity is no
+//    number: then the wave sweeps once more.
 //  * End of a segment: the waves' (O, m, l) meet in LDS.  A unit that is one
 //    segment is written out; otherwise each of its workgroups leaves its part
-//    in the workspace and counts itself in, and the last one joins the parts in
-//    their order and puts the counter back to zero.  Nobody waits for another
-//    workgroup.
+//    in the workspace and counts itself in, and the last of every eight
+//    neighbours joins them, and so on up.  Nobody waits for another workgroup.
 #pragma once
 
 #include "paged_common.h"

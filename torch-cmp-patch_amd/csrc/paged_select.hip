@@ -9,15 +9,21 @@
 //
 // paged_scores reads every page's bounds once and is bound by that: 8 to 64
 // lanes take a page (a 16-byte chunk of lo and of hi each, its Q+ and Q- in
-// registers), four steps of pages in flight.
+// registers), four steps of pages in flight (measured on MI355X: 8 heads x 8192
+// pages of 128 fp16 channels 9.8 us, 3.4 TB/s; 20.1 us with the choice, 22.6 with
+// two steps in flight, 20.1 with eight).
 //
 // paged_best takes the best of each (sequence, head) with one workgroup, whose
-// waves hold a range of columns each.  The border is found by histograms:
-// the range of the keys still in question is cut into 2048 equal bins, the bin
-// that holds the border is the next range (scores of one magnitude spread
-// evenly over it: two rounds for most inputs).  Which columns are taken is
-// then a ballot per 64 columns, so they are written in ascending order, equal
-// scores from the lowest column on.
+// waves hold a range of columns each.  The border is found by histograms of 2048
+// bins: first 256 an octave around one of the scores, then, while more than 64
+// scores share the border's bin, the range of those in equal parts; 64 or fewer
+// are ranked by comparing all with all.  Which columns are taken is then a
+// ballot per 64 columns, so they are written in ascending order, equal scores
+// from the lowest column on.  8.9 us for 8 rows of 8192 (latency: barriers and
+// LDS atomics of one workgroup a row).
+//
+// paged_short does both for rows of up to 1024 pages, a workgroup a row: 9.5 us
+// for 16 x 8 rows of 256 pages, 12.2 in two launches.
 #include "paged_common.h"
 
 namespace cmpext3 {
