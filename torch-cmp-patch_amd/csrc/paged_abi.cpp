@@ -221,6 +221,7 @@ int cmpext3_paged_select(const void* q, const void* key_bounds, int32_t* selecte
   p.kb_p = kb_str[0]; p.kb_h = kb_str[1]; p.kb_e = kb_str[2];
   p.B = B; p.H = H; p.Hkv = H_kv; p.D = D;
   p.map = map_of(page_table, table_width, table_stride, seq_lens, nullptr, num_pages, page_size);
+  p.by_ps = cmpext3::div_by(page_size);
   p.n_selected = n_selected;
   p.workspace = workspace;
   std::unique_lock<std::mutex> submit(cmpext3::space_lock(workspace), std::defer_lock);

@@ -5,6 +5,21 @@
 
 namespace cmpext3 {
 
+// n / d for 0 <= n < 2^31 as a product: s = ceil(log2 d), m = floor(2^(31+s) / d)
+// + 1 exceeds the quotient's scale by less than 2^s / 2^(31+s), too little to
+// reach the next whole number.
+struct Div {
+  uint32_t m;
+  int s;
+};
+__device__ __forceinline__ int quot(int n, uint32_t m, int s) { return (int)(__umulhi((uint32_t)n << 1, m) >> s); }
+
+inline Div div_by(int d) {
+  int s = 0;
+  while ((1ll << s) < d) ++s;
+  return {(uint32_t)((1ull << (31 + s)) / (uint32_t)d + 1), s};
+}
+
 // The sequences' pages and lengths (all on the device).
 struct PageMap {
   const int32_t* table;  // [B][width], row stride `stride`
@@ -49,6 +64,7 @@ struct SelectParams {
   int64_t q_b, q_h, kb_p, kb_h, kb_e;
   int B, H, Hkv, D;
   PageMap map;
+  Div by_ps;
   int n_selected;
   void* workspace;
 };
@@ -58,21 +74,6 @@ hipError_t launch_paged_attn(const PagedAttnParams& p, int dtype, hipStream_t s)
 size_t paged_attn_workspace(int dtype, int B, int H, int Hkv, int S, int D, int page_size, int width, int n_selected);
 hipError_t launch_paged_select(const SelectParams& p, int dtype, hipStream_t s);
 size_t paged_select_workspace(int B, int Hkv, int width);
-
-// n / d for 0 <= n < 2^31 as a product: s = ceil(log2 d), m = floor(2^(31+s) / d)
-// + 1 exceeds the quotient's scale by less than 2^s / 2^(31+s), too little to
-// reach the next whole number.
-struct Div {
-  uint32_t m;
-  int s;
-};
-__device__ __forceinline__ int quot(int n, uint32_t m, int s) { return (int)(__umulhi((uint32_t)n << 1, m) >> s); }
-
-inline Div div_by(int d) {
-  int s = 0;
-  while ((1ll << s) < d) ++s;
-  return {(uint32_t)((1ull << (31 + s)) / (uint32_t)d + 1), s};
-}
 
 __device__ __forceinline__ int block_y() { return (int)__builtin_amdgcn_workgroup_id_y(); }
 __device__ __forceinline__ int block_z() { return (int)__builtin_amdgcn_workgroup_id_z(); }

@@ -22,7 +22,7 @@
 // from the lowest column on.  8.9 us for 8 rows of 8192 (latency: barriers and
 // LDS atomics of one workgroup a row).
 //
-// paged_short does both for rows of up to 1024 pages, a workgroup a row: 9.5 us
+// paged_short does both for rows of up to 1024 pages, a workgroup a row: 9.0 us
 // for 16 x 8 rows of 256 pages, 12.2 in two launches.
 #include "paged_common.h"
 
@@ -43,8 +43,8 @@ __device__ __forceinline__ uint64_t order_of(double x) {
 }
 
 // Pages of sequence b that its table row holds.
-__device__ __forceinline__ int pages_of(const PageMap& m, int b) {
-  return min((seq_len_held(m, b) + m.page_size - 1) / m.page_size, m.width);
+__device__ __forceinline__ int pages_of(const SelectParams& p, int b) {
+  return min(quot(seq_len_held(p.map, b) + p.map.page_size - 1, p.by_ps.m, p.by_ps.s), p.map.width);
 }
 
 // Element e of a 16-byte chunk.
@@ -101,18 +101,22 @@ struct Weights {
   }
 };
 
-// The bounds of kSteps steps of 64 / LG pages from this lane's column col0 on, on
-// their way while the weights are made.
+// The bounds of kSteps steps of 64 / LG pages from this lane's column col0 on: the
+// page numbers are on their way before the sequence's length is known, the
+// bounds while the weights are made.
 template <typename T, int LG>
 struct Bounds {
   int page[kSteps];
   u32x4 lo[kSteps], hi[kSteps];
-  __device__ __forceinline__ void load(const SelectParams& p, int b, int hk, int col0, int pages, int c) {
+  __device__ __forceinline__ void look(const SelectParams& p, int b, int col0) {
+#pragma unroll
+    for (int s = 0; s < kSteps; ++s) page[s] = page_at(p.map, b, col0 + s * (64 / LG));
+  }
+  __device__ __forceinline__ void load(const SelectParams& p, int hk, int col0, int pages, int c) {
     constexpr int N = 16 / sizeof(T), PW = 64 / LG;
 #pragma unroll
-    for (int s = 0; s < kSteps; ++s) page[s] = col0 + s * PW < pages ? page_at(p.map, b, col0 + s * PW) : -1;
-#pragma unroll
     for (int s = 0; s < kSteps; ++s) {
+      if (col0 + s * PW >= pages) page[s] = -1;
       lo[s] = hi[s] = (u32x4){0u, 0u, 0u, 0u};
       if (c * N < p.D && page[s] >= 0) {
         const T* at = (const T*)p.bounds + page[s] * p.kb_p + hk * p.kb_h + c * N;
@@ -125,15 +129,15 @@ struct Bounds {
 
 // put(column, key) of those pages.
 template <typename T, int LG, typename Put>
-__device__ __forceinline__ void score_pages(const Bounds<T, LG>& bd, const Weights<T>& w, int col0, int pages, Put put) {
+__device__ __forceinline__ void score_pages(const Bounds<T, LG>& read, const Weights<T>& w, int col0, int pages, Put put) {
   constexpr int N = Weights<T>::N, PW = 64 / LG;
 #pragma unroll
   for (int s = 0; s < kSteps; ++s) {
     double sum = 0;
 #pragma unroll
     for (int e = 0; e < N; ++e) {
-      sum = __builtin_fma(w.up[e], (double)elem<T>(bd.hi[s], e), sum);
-      sum = __builtin_fma(w.down[e], (double)elem<T>(bd.lo[s], e), sum);
+      sum = __builtin_fma(w.up[e], (double)elem<T>(read.hi[s], e), sum);
+      sum = __builtin_fma(w.down[e], (double)elem<T>(read.lo[s], e), sum);
     }
     sum = group_sum<LG>(sum);
     if (__builtin_amdgcn_ballot_w64(sum != sum)) {
@@ -141,14 +145,14 @@ __device__ __forceinline__ void score_pages(const Bounds<T, LG>& bd, const Weigh
       double t = 0;
 #pragma unroll
       for (int e = 0; e < N; ++e) {
-        if (w.up[e] != 0) t = __builtin_fma(w.up[e], (double)elem<T>(bd.hi[s], e), t);
-        if (w.down[e] != 0) t = __builtin_fma(w.down[e], (double)elem<T>(bd.lo[s], e), t);
+        if (w.up[e] != 0) t = __builtin_fma(w.up[e], (double)elem<T>(read.hi[s], e), t);
+        if (w.down[e] != 0) t = __builtin_fma(w.down[e], (double)elem<T>(read.lo[s], e), t);
       }
       t = group_sum<LG>(t);
       if (sum != sum) sum = t;
     }
     const int col = col0 + s * PW;
-    if (w.c == 0 && col < pages) put(col, bd.page[s] >= 0 ? order_of(sum) : kBest);
+    if (w.c == 0 && col < pages) put(col, read.page[s] >= 0 ? order_of(sum) : kBest);
   }
 }
 
@@ -157,11 +161,12 @@ __global__ __launch_bounds__(256) void paged_scores(SelectParams p, uint64_t* ke
   constexpr int PW = 64 / LG;        // pages of a wave's step
   const int hk = block_y(), b = block_z();
   const int lane = thread_x() & 63, wave = thread_x() >> 6;
-  const int pages = pages_of(p.map, b);
-  if (block_x() * 4 * kSteps * PW >= pages) return;
   const int col0 = (block_x() * 4 + wave) * kSteps * PW + lane / LG;
   Bounds<T, LG> e;
-  e.load(p, b, hk, col0, pages, lane & (LG - 1));
+  e.look(p, b, col0);
+  const int pages = pages_of(p, b);
+  if (block_x() * 4 * kSteps * PW >= pages) return;
+  e.load(p, hk, col0, pages, lane & (LG - 1));
   Weights<T> w;
   w.load(p, b, hk, lane & (LG - 1));
   uint64_t* row = keys + ((int64_t)b * p.Hkv + hk) * p.map.width;
@@ -175,6 +180,13 @@ __device__ __forceinline__ uint64_t wave_min(uint64_t x) {
     x = o < x ? o : x;
   }
   return x;
+}
+
+// Sum of the waves' numbers before this wave's.
+template <int NW>
+__device__ __forceinline__ int before_wave(const int* sums, int lane, int wave) {
+  const int v = lane < NW ? sums[lane] : 0;
+  return __builtin_amdgcn_readlane(wave_scan(v) - v, __builtin_amdgcn_readfirstlane(wave));
 }
 
 struct BestShared {
@@ -254,8 +266,7 @@ __device__ __forceinline__ void best(BestShared& sh, int pages, int K, int32_t* 
         each([&](uint64_t k, int) { eq += __builtin_popcountll(__builtin_amdgcn_ballot_w64(k == lo)); });
         if (lane == 0) sh.sum[wave] = eq;
         __syncthreads();
-        int before = 0;
-        for (int w = 0; w < wave; ++w) before += sh.sum[w];
+        int before = before_wave<NW>(sh.sum, lane, wave);
         if (before < need && before + eq >= need)
           each([&](uint64_t k, int c) {
             const uint64_t in = __builtin_amdgcn_ballot_w64(k == lo);
@@ -293,8 +304,7 @@ __device__ __forceinline__ void best(BestShared& sh, int pages, int K, int32_t* 
     if (lane == 63) sh.sum[wave] = inc;
     if (tid == 0) sh.cands = 0;
     __syncthreads();
-    int above = inc - mine;
-    for (int w = 0; w < wave; ++w) above += sh.sum[w];
+    int above = inc - mine + before_wave<NW>(sh.sum, lane, wave);
 #pragma unroll
     for (int j = 0; j < BT; ++j) {
       if (above < need && above + h[j] >= need) {
@@ -359,8 +369,7 @@ __device__ __forceinline__ void best(BestShared& sh, int pages, int K, int32_t* 
   __syncthreads();
   if (lane == 0) sh.sum[wave] = before;
   __syncthreads();
-  before = 0;
-  for (int w = 0; w < wave; ++w) before += sh.sum[w];
+  before = before_wave<NW>(sh.sum, lane, wave);
   each([&](uint64_t k, int c) {
     const uint64_t in = __builtin_amdgcn_ballot_w64(taken(k, c));
     if (taken(k, c)) out[before + __builtin_popcountll(in & (lane ? ~0ull >> (64 - lane) : 0ull))] = c;
@@ -373,7 +382,7 @@ __global__ __launch_bounds__(NW * 64) void paged_best(SelectParams p, const uint
   __shared__ BestShared sh;
   const int hk = block_x(), b = block_y();
   const uint64_t* keys = all + ((int64_t)b * p.Hkv + hk) * p.map.width;
-  best<NW, HELD>(sh, pages_of(p.map, b), p.n_selected, p.selected + ((int64_t)b * p.Hkv + hk) * p.n_selected,
+  best<NW, HELD>(sh, pages_of(p, b), p.n_selected, p.selected + ((int64_t)b * p.Hkv + hk) * p.n_selected,
                  [&](int c) { return keys[c]; });
 }
 
@@ -385,16 +394,20 @@ __global__ __launch_bounds__(1024) void paged_short(SelectParams p) {
   constexpr int PW = 64 / LG;
   const int hk = block_x(), b = block_y();
   const int lane = thread_x() & 63, wave = thread_x() >> 6;
-  const int pages = pages_of(p.map, b);
+  Bounds<T, LG> e;
+  e.look(p, b, wave * kSteps * PW + lane / LG);
+  const int pages = pages_of(p, b);
   if (pages > p.n_selected && p.n_selected > 1) {
-    Bounds<T, LG> e;
-    e.load(p, b, hk, wave * kSteps * PW + lane / LG, pages, lane & (LG - 1));
+    e.load(p, hk, wave * kSteps * PW + lane / LG, pages, lane & (LG - 1));
     Weights<T> w;
     w.load(p, b, hk, lane & (LG - 1));
     for (int c0 = wave * kSteps * PW; c0 < pages;) {
       score_pages<T, LG>(e, w, c0 + lane / LG, pages, [&](int c, uint64_t k) { keys[c] = k; });
       c0 += 16 * kSteps * PW;
-      if (c0 < pages) e.load(p, b, hk, c0 + lane / LG, pages, lane & (LG - 1));
+      if (c0 < pages) {
+        e.look(p, b, c0 + lane / LG);
+        e.load(p, hk, c0 + lane / LG, pages, lane & (LG - 1));
+      }
     }
     __syncthreads();
   }
