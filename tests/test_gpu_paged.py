@@ -593,6 +593,43 @@ def test_refusals():
         att(q=q.clone().requires_grad_())
 
 
+# how the tables lie in memory: half of doubled ones, a column in two, transposed, one row for all, unlike each other
+TABLES = {
+    "halves": lambda t: (torch.cat([t[0], t[0]], 1)[:, :t[0].shape[1]], torch.cat([t[1], t[1]], 1)[:, :t[0].shape[1]]),
+    "one pair of tensors": lambda t: torch.cat(t, 1).chunk(2, 1),
+    "from an odd word": lambda t: tuple(torch.cat([x[:, :1], x], 1)[:, 1:] for x in t),
+    "spread": lambda t: tuple(x.repeat_interleave(2, 1)[:, ::2] for x in t),
+    "transposed": lambda t: tuple(x.t().contiguous().t() for x in t),
+    "mixed": lambda t: (torch.cat([t[0], t[0]], 1)[:, :t[0].shape[1]], t[1]),
+    "one row": lambda t: tuple(x[7:8].expand_as(x) for x in t),
+}
+
+
+@pytest.mark.parametrize("lies", TABLES)
+@pytest.mark.parametrize("dtype,rot,pairs", [("bf16", 64, False), ("fp16", 24, True), ("fp32", 12, False), ("fp32", 2, False)])
+def test_rotation_tables_of_any_layout(dtype, rot, pairs, lies):
+    c = Cache(dtype, [70, 33], 2, 64, 16)
+    k, v, q = c.rows(2, 9), c.rows(2, 9), c.rows(4, 9)
+    cos, sin = TABLES[lies](tables(80, rot))
+    out = []
+    for t in ((cos, sin), (cos.contiguous(), sin.contiguous())):
+        kp, vp = torch.zeros_like(c.kp), torch.zeros_like(c.vp)
+        out.append((cmpext3.paged_append(k, v, kp, vp, c.table, c.lens, query=q, cos=t[0], sin=t[1], interleaved=pairs), kp, vp))
+    assert all(torch.equal(a, b) for a, b in zip(*out)) and not out[0][0].isnan().any()
+
+
+def test_tables_that_are_learned_are_refused():
+    c = Cache("bf16", [50, 20], 2, 64, 16)
+    k = c.rows(2, 1)
+    for i in range(2):
+        t = list(tables(64, 64))
+        t[i].requires_grad_()
+        with pytest.raises(RuntimeError, match="no backward"):
+            cmpext3.paged_append(k, k, c.kp, c.vp, c.table, c.lens, cos=t[0], sin=t[1])
+        with torch.no_grad():
+            cmpext3.paged_append(k, k, c.kp, c.vp, c.table, c.lens, cos=t[0], sin=t[1])
+
+
 # dtype, lens, H, Hkv, D, page, S: shares that span units, units cut by themselves, whole units
 SPLITS = [
     ("bf16", [5000, 70, 0, 2600], 8, 2, 128, 16, 1),

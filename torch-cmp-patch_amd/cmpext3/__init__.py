@@ -204,7 +204,8 @@ def paged_append(key: torch.Tensor, value: torch.Tensor, key_pages: torch.Tensor
                  columns are padding; by default every column is new (the first seq_lens[b], if fewer)
     cos, sin     fp32 [rows, R / 2]: keys and queries [B, H, S, D] are rotated in their first R dims by
                  row positions[b, i] (int32 [B, S]; the token's place in its sequence by default), as
-                 pairs (d, d + R/2), or (2d, 2d + 1) when `interleaved`
+                 pairs (d, d + R/2), or (2d, 2d + 1) when `interleaved`; columns of wider tables are
+                 read in place where both have the same row stride
     key_bounds   [pages, Hkv, 2, D]: every channel's lowest and highest key of a page, kept up to date
                  for paged_select
 

@@ -133,20 +133,25 @@ static c10::optional<torch::Tensor> paged_append(
   TORCH_CHECK(!given(query) || given(cos), "cmpext3 paged: query is there to be rotated: cos and sin are missing");
   TORCH_CHECK(!given(positions) || given(cos), "cmpext3 paged: positions name rows of cos and sin, which are missing");
   const torch::Tensor none;
-  check_grad({&key, &value, &key_pages, &value_pages, given(query) ? &*query : &none,
-              given(key_bounds) ? &*key_bounds : &none});
+  check_grad({&key, &value, &key_pages, &value_pages, given(query) ? &*query : &none, given(cos) ? &*cos : &none,
+              given(sin) ? &*sin : &none, given(key_bounds) ? &*key_bounds : &none});
   torch::Tensor c, s, at_rows, q, out;
   int rows = 0, rot = 0;
+  int64_t row_stride = 0;
   if (given(cos)) {
     TORCH_CHECK(cos->dim() == 2 && cos->sizes() == sin->sizes() && cos->scalar_type() == at::kFloat &&
                     sin->scalar_type() == at::kFloat && cos->device() == key.device() && sin->device() == key.device(),
                 "cmpext3 paged: cos and sin must be fp32 [rows, rotated dims / 2] on key's device");
     TORCH_CHECK(cos->size(0) >= 1 && cos->size(0) <= INT32_MAX && cos->size(1) >= 1 && 2 * cos->size(1) <= D,
                 "cmpext3 paged: cos and sin rotate ", 2 * cos->size(1), " of ", D, " dims");
-    c = cos->contiguous();
-    s = sin->contiguous();
+    // rows of wider tables (half of [cos, cos], say) are read where they lie
+    const bool as_is = cos->stride(0) == sin->stride(0) &&
+                       (cos->size(1) == 1 || (cos->stride(1) == 1 && sin->stride(1) == 1));
+    c = as_is ? *cos : cos->contiguous();
+    s = as_is ? *sin : sin->contiguous();
     rows = (int)c.size(0);
     rot = 2 * (int)c.size(1);
+    row_stride = rows > 1 ? c.stride(0) : 0;
   }
   if (given(positions)) {
     check_ints("positions", *positions, key, {B, S});
@@ -182,7 +187,7 @@ static c10::optional<torch::Tensor> paged_append(
                (int)P, (int)page, ks.s, vs.s, qs.s, os.s, kps.s, vps.s, kbs.s, map.pages(), map.width, map.stride,
                map.lens.data_ptr<int32_t>(), map.news(),
                at_rows.defined() ? at_rows.data_ptr<int32_t>() : nullptr, rot ? c.data_ptr<float>() : nullptr,
-               rot ? s.data_ptr<float>() : nullptr, rows, rot, rot / 2, interleaved ? 1 : 0, stream_of(key)),
+               rot ? s.data_ptr<float>() : nullptr, rows, rot, row_stride, interleaved ? 1 : 0, stream_of(key)),
            "paged_append");
   wrote(key_pages);
   wrote(value_pages);
