@@ -1,5 +1,5 @@
 """Float64 restatement of the paged key-value cache's operators, used as the
-checker on the CPU: plain loops over sequences, heads and tokens, following
+oracle on the CPU: plain loops over sequences, heads and tokens, following
 include/cmpext3_paged.h word for word."""
 from __future__ import annotations
 

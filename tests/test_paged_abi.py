@@ -118,7 +118,7 @@ def test_cpu_tensors_are_refused():
 
 
 def test_the_float64_restatement_is_plain_attention():
-    """The checker itself: over an identity table it is softmax attention with a causal corner, and its page scores
+    """The oracle itself: over an identity table it is softmax attention with a causal corner, and its page scores
     bound every key's product."""
     g = torch.Generator().manual_seed(0)
     q = torch.randn(1, 4, 3, 8, generator=g, dtype=torch.float64)

@@ -10,8 +10,8 @@
 // paged_scores reads every page's bounds once and is bound by that: 8 to 64
 // lanes take a page (a 16-byte chunk of lo and of hi each, its Q+ and Q- in
 // registers), four steps of pages in flight (measured on MI355X: 8 heads x 8192
-// pages of 128 fp16 channels 9.8 us, 3.4 TB/s; 20.1 us with the choice, 22.6 with
-// two steps in flight, 20.1 with eight).
+// pages of 128 fp16 channels 10.2 us, 3.3 TB/s; with the choice 19.5 us, and 20.1
+// before it got faster, against 22.6 with two steps in flight and 20.1 with eight).
 //
 // paged_best takes the best of each (sequence, head) with one workgroup, whose
 // waves hold a range of columns each.  The border is found by histograms of 2048
@@ -19,11 +19,11 @@
 // scores share the border's bin, the range of those in equal parts; 64 or fewer
 // are ranked by comparing all with all.  Which columns are taken is then a
 // ballot per 64 columns, so they are written in ascending order, equal scores
-// from the lowest column on.  8.9 us for 8 rows of 8192 (latency: barriers and
+// from the lowest column on.  7.5 us for 8 rows of 8192 (latency: barriers and
 // LDS atomics of one workgroup a row).
 //
-// paged_short does both for rows of up to 1024 pages, a workgroup a row: 9.0 us
-// for 16 x 8 rows of 256 pages, 12.2 in two launches.
+// paged_short does both for rows of up to 1024 pages, a workgroup a row: 9.5 us
+// for 16 x 8 rows of 256 pages (10.0 with the call's own; 12.2 in two launches).
 #include "paged_common.h"
 
 namespace cmpext3 {
@@ -322,8 +322,8 @@ __device__ __forceinline__ void best(BestShared& sh, int pages, int K, int32_t* 
       lo += (uint64_t)bin << shift;
       hi = top < hi && top >= lo ? top : hi;
     } else {  // the outermost bins hold all that lies beyond them
-      if (bin < kBins - 1) hi = (uint64_t)((zero + bin + 1) << 44) - 1;
-      if (bin > 0) lo = (uint64_t)((zero + bin) << 44);
+      if (bin < kBins - 1) hi = ((uint64_t)(zero + bin + 1) << 44) - 1;
+      if (bin > 0) lo = (uint64_t)(zero + bin) << 44;
     }
     if (inside == need) {  // all of the bin
       key = lo - 1;
