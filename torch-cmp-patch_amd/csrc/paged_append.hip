@@ -2,8 +2,8 @@
 // embedding applied on the way.
 //
 // Bound by HBM for prompts (every row is read once and written once; measured on
-// MI355X: bf16 4 x 2048 tokens of 16 + 8 + 8 heads of 128 with bounds 30.9 us,
-// 4.4 TB/s) and by the latency of its loads for single tokens (16 of them 3.3
+// MI355X: bf16 4 x 2048 tokens of 16 + 8 + 8 heads of 128 with bounds 30.3 us,
+// 4.5 TB/s) and by the latency of its loads for single tokens (16 of them 3.3
 // us): lengths, then the page number and the rotation's row, while the rows
 // themselves, which depend on neither, are on their way.
 //
@@ -264,7 +264,9 @@ __device__ __forceinline__ void append_run(const AppendParams& p, const Shape& s
   r1.clear();
   bool some = false;
   if (t < TL) {
-#pragma unroll 2
+    // one step at a time: a second in flight takes more registers than it hides
+    // (bf16 4 x 2048 tokens 31.3 us with two, 30.3 with one; 8 x 80 8.4, 8.1)
+#pragma unroll 1
     for (int i = i0 + t + (WAVES == 1 ? 0 : wave * TL); i < i1; i += TL * WAVES) {
       const T* row = src + i * p.k_s;
       Unit<T, MODE> w = at;
